@@ -26,6 +26,7 @@ from .api import (  # noqa: F401
     gemmGPU,
     quantize_rowwise,
     quantize_block,
+    rmsnorm_quantize,
     HostContext,
     select_path,
     select_path_sms,

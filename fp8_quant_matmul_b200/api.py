@@ -63,6 +63,8 @@ _SIGS = {
     "fp8bs_gemm_host": (_c.c_int, [_c.c_void_p] * 6 + [_c.c_int] * 5),
     "fp8bs_quantize_rowwise": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int, _c.c_float, _c.c_void_p]),
     "fp8bs_quantize_block": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int, _c.c_float, _c.c_void_p]),
+    "fp8bs_rmsnorm_quantize": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_longlong, _c.c_void_p, _c.c_int, _c.c_longlong, _c.c_void_p, _c.c_void_p,
+                                          _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int, _c.c_float, _c.c_float, _c.c_void_p]),
     "fp8bs_gen_normal_e4m3": (_c.c_int, [_c.c_void_p, _c.c_size_t, _c.c_uint64]),
     "fp8bs_gen_uniform_f32": (_c.c_int, [_c.c_void_p, _c.c_size_t, _c.c_uint64, _c.c_float, _c.c_float]),
     "fp8bs_float_to_e4m3fn": (_c.c_uint8, [_c.c_float]),
@@ -399,6 +401,68 @@ def quantize_block(W, fp8_max=448.0):
     """B and b_scale of the GEMM from a row-major [N, K] weight matrix (128 x 128 blocks, quantize.py:16-41).
     Returns (B bytes column-major, flat; inverse scales laid out b_scale[nb + ceil(N/128)*kb])."""
     return _quantize("fp8bs_quantize_block", W, fp8_max)
+
+
+def _call(name, index, *args):
+    """A library call for tensors of CUDA device `index`, on that device's current stream."""
+    torch = _torch()
+    fn = getattr(lib(), name)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _stream(index))
+    else:                                           # the library launches on the current device
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
+    if rc != 0:
+        _check(rc, name)
+
+
+def _is_bf16(dtype, what):
+    torch = _torch()
+    if dtype is torch.bfloat16:
+        return 1
+    if dtype is torch.float32:
+        return 0
+    raise ValueError("%s has to be fp32 or bf16" % what)
+
+
+def rmsnorm_quantize(X, weight, residual=None, eps=1e-6, fp8_max=448.0, residual_out=None):
+    """A and a_scale of the GEMM from the root-mean-square norm of X [rows, K], or of X + residual, in one launch.
+
+        s = X + residual;  y = s / sqrt(mean(s^2) + eps) * weight   (fp32);  then the scaling of quantize_rowwise
+
+    Returns (A bytes column-major, flat; inverse scales, flat) for M = rows rounded up to a multiple of 16, the rows behind the last
+    being zeros; with a residual also s in the residual's type, in residual_out if that is given (which may be the residual, or X).
+    X, residual and weight: fp32 or bf16 each.  X and residual may be column slices (any row stride of whole 16 bytes).
+    """
+    torch = _torch()
+    if not X.is_cuda or X.dim() != 2 or X.stride(1) != 1:
+        raise ValueError("X has to be a 2-D CUDA tensor [rows, K] with contiguous rows")
+    rows, K = X.shape
+    index = X.get_device()
+    if weight.shape != (K,) or weight.get_device() != index or not weight.is_contiguous():
+        raise ValueError("weight has to be a contiguous tensor [K] on X's device")
+    x_bf16, w_bf16, r_bf16 = _is_bf16(X.dtype, "X"), _is_bf16(weight.dtype, "weight"), 0
+    r_ptr = out_ptr = None
+    ldr = K
+    if residual is not None:
+        if residual.shape != X.shape or residual.get_device() != index or residual.stride(1) != 1:
+            raise ValueError("residual has to be a tensor like X, on its device, with contiguous rows")
+        r_bf16 = _is_bf16(residual.dtype, "residual")
+        if residual_out is None:
+            residual_out = torch.empty((rows, K), dtype=residual.dtype, device=X.device)
+        elif (residual_out.shape != X.shape or residual_out.dtype is not residual.dtype or residual_out.get_device() != index
+              or not residual_out.is_contiguous()):
+            raise ValueError("residual_out has to be a contiguous tensor [rows, K] of the residual's type on X's device")
+        r_ptr, out_ptr = residual.data_ptr(), residual_out.data_ptr()
+        ldr = residual.stride(0) if rows > 1 else K
+    elif residual_out is not None:
+        raise ValueError("residual_out without a residual")
+    M = (rows + 15) // 16 * 16
+    q = torch.empty(M * K, dtype=torch.uint8, device=X.device)
+    scales = torch.empty(M * (K // 128), dtype=torch.float32, device=X.device)
+    _call("fp8bs_rmsnorm_quantize", index, X.data_ptr(), x_bf16, X.stride(0) if rows > 1 else K, r_ptr, r_bf16, ldr, out_ptr,
+          weight.data_ptr(), w_bf16, q.data_ptr(), scales.data_ptr(), rows, K, eps, fp8_max)
+    return (q, scales) if residual is None else (q, scales, residual_out)
 
 
 def last_device_status(stream=None):

@@ -5,6 +5,7 @@
 #include "gemm_kernel.cuh"
 #include "gemm_small_m.cuh"
 #include "quantize.cuh"
+#include "rmsnorm.cuh"
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -615,6 +616,55 @@ static int launch_small_m(const TensorMaps& tm, const GemmParams& p, cudaStream_
 {
     using Cfg = SmallMCfg<T>;
     return launch_clusters(gemm_small_m_kernel<T>, p.n_tiles * p.splits, p.splits, Cfg::THREADS, Cfg::SMEM_BYTES, stream, tm.A, tm.B, p);
+}
+
+// How many clusters of `cluster` CTAs with `warps` warps of the norm kernel run at once: asked once per device, type and shape.
+template <class X, class R>
+static int norm_clusters(int device, int cluster, int warps, int smem, int* out)
+{
+    static std::atomic<int> known[MAX_DEVICES][NORM_MAX_CLUSTER + 1][NORM_MOST_WARPS + 1];
+    std::atomic<int>& slot = known[device][cluster][warps];
+    int n = slot.load(std::memory_order_relaxed);
+    if (n == 0) {
+        CUDA_TRY(cudaFuncSetAttribute(rmsnorm_quantize_kernel<X, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_SMEM_LIMIT + NORM_FIXED_SMEM));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(cluster * 64), 1, 1);
+        cfg.blockDim = dim3(static_cast<unsigned>(32 * warps), 1, 1);
+        cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, rmsnorm_quantize_kernel<X, R>, &cfg));
+        if (n < 1) return FP8BS_ERR_NO_DEVICE;
+        slot.store(n, std::memory_order_relaxed);
+    }
+    *out = n;
+    return FP8BS_OK;
+}
+
+template <class X, class R>
+static int launch_rmsnorm(NormParams p, const DeviceInfo* dev, cudaStream_t st)
+{
+    // As few CTAs per cluster as hold the row, and as few warps in each (K = 2304: 3 x 6 instead of 3 x 8).
+    const int KB = p.K / 128, groups = p.M / NORM_ROWS;
+    const int cluster = std::min(ceil_div(KB, NORM_WARPS), NORM_MAX_CLUSTER), warps = ceil_div(KB, cluster);
+    int element = sizeof(X);
+    if constexpr (!std::is_void<R>::value) element += sizeof(R);
+    const long long buffers = static_cast<long long>(NORM_ROWS) * 128 * warps * element;
+    if (warps > NORM_MOST_WARPS || buffers > NORM_SMEM_LIMIT)
+        return launch_grid(rmsnorm_quantize_long_kernel<X, R>, dim3(static_cast<unsigned>(groups * NORM_MAX_CLUSTER), 1, 1), NORM_MAX_CLUSTER,
+                           32 * NORM_WARPS, 0, st, p);
+    const int smem = static_cast<int>(buffers) + NORM_FIXED_SMEM;
+    int most = 0;
+    const int rc = norm_clusters<X, R>(static_cast<int>(dev - g_dev), cluster, warps, smem, &most);
+    if (rc) return rc;
+    p.cluster = cluster;
+    return launch_grid(rmsnorm_quantize_kernel<X, R>, dim3(static_cast<unsigned>(std::min(groups, most) * cluster), 1, 1), cluster, 32 * warps, smem,
+                       st, p);
 }
 
 static int launch_config(const Config& c, const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t st)
@@ -1548,6 +1598,42 @@ int fp8bs_quantize_block(const void* W, int w_is_bf16, void* B_out, float* b_sca
                          void* stream)
 {
     return quantize_impl(true, W, w_is_bf16, B_out, b_scale_out, N, K, fp8_max, stream);
+}
+
+// ---- norm in front of the quantiser --------------------------------------------------------------
+int fp8bs_rmsnorm_quantize(const void* X, int x_is_bf16, long long ldx, const void* residual, int r_is_bf16, long long ldr,
+                           void* residual_out, const void* weight, int w_is_bf16, void* A_out, float* a_scale_out, int rows,
+                           int K, float eps, float fp8_max, void* stream)
+{
+    if (!X || !weight || !A_out || !a_scale_out || (residual && !residual_out)) return FP8BS_ERR_NULL;
+    if (rows <= 0 || rows > 0x7ffffff0 || K <= 0 || K % 128 != 0) return FP8BS_ERR_SHAPE;
+    if (ldx < K || (residual && ldr < K)) return FP8BS_ERR_ARG;
+    auto off = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) != 0; };
+    if (off(X) || off(weight) || ldx % (x_is_bf16 ? 8 : 4) != 0) return FP8BS_ERR_ALIGN;      // every row starts on 16 bytes
+    if (residual && (off(residual) || off(residual_out) || ldr % (r_is_bf16 ? 8 : 4) != 0)) return FP8BS_ERR_ALIGN;
+    if (off(A_out) || (reinterpret_cast<uintptr_t>(a_scale_out) & 3u)) return FP8BS_ERR_ALIGN;
+    if (!(fp8_max > 0.0f) || fp8_max > 448.0f || !(eps >= 0.0f)) return FP8BS_ERR_ARG;
+    const long long groups = (static_cast<long long>(rows) + 15) / 16;
+    if (groups * NORM_MAX_CLUSTER > 0x7fffffff) return FP8BS_ERR_SHAPE;
+    DeviceInfo* dev = nullptr;
+    const int rc = device_setup(&dev);
+    if (rc) return rc;
+    NormParams p;
+    p.x = X; p.r = residual; p.r_out = residual_out; p.w = weight;
+    p.out = static_cast<uint8_t*>(A_out);
+    p.scale_out = a_scale_out;
+    p.ldx = ldx; p.ldr = ldr;
+    p.rows = rows; p.M = static_cast<int>(groups * 16); p.K = K;
+    p.status = dev->status_ptr;
+    p.cluster = 0;
+    p.w_is_bf16 = w_is_bf16;
+    p.eps = eps; p.fp8_max = fp8_max;
+    p.clamp = host_e4m3fn_to_float(float_to_e4m3fn_rne(fp8_max)) != fp8_max;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    using bf16 = __nv_bfloat16;
+    if (!residual) return x_is_bf16 ? launch_rmsnorm<bf16, void>(p, dev, st) : launch_rmsnorm<float, void>(p, dev, st);
+    if (r_is_bf16) return x_is_bf16 ? launch_rmsnorm<bf16, bf16>(p, dev, st) : launch_rmsnorm<float, bf16>(p, dev, st);
+    return x_is_bf16 ? launch_rmsnorm<bf16, float>(p, dev, st) : launch_rmsnorm<float, float>(p, dev, st);
 }
 
 // ---- generators / conversions (host only) -------------------------------------------------

@@ -92,6 +92,13 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm,
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(bar)
         : "memory");
 }
+// Untiled copy global -> shared of this CTA, counted in bytes on `bar`.  Both addresses and the size: multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 // 2-D tiled store shared -> global (bulk-group completion).
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, uint32_t src, int c0, int c1)
 {
@@ -189,6 +196,13 @@ __device__ __forceinline__ void cluster_wait()
 __device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, float v)
 {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+// The same without waiting for it to land: the four bytes are counted on `cluster_bar`, a barrier of the receiving CTA.
+__device__ __forceinline__ void st_async_f32(uint32_t cluster_addr, float v, uint32_t cluster_bar)
+{
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];"
+                 ::"r"(cluster_addr), "r"(__float_as_uint(v)), "r"(cluster_bar)
+                 : "memory");
 }
 // 16 bytes from the shared memory of any CTA of the cluster (address from mapa).
 __device__ __forceinline__ float4 ld_shared_cluster_v4(uint32_t cluster_addr)

@@ -220,6 +220,21 @@ int fp8bs_quantize_rowwise(const void* X, int x_is_bf16, void* A_out, float* a_s
 int fp8bs_quantize_block(const void* W, int w_is_bf16, void* B_out, float* b_scale_out, int N, int K,
                          float fp8_max, void* stream);
 
+/* Root-mean-square norm with the residual's addition in front of it and the GEMM's A operand behind it, one launch:
+ *     s = X + residual (fp32);  residual_out = s in the residual's type;  y = s / sqrt(mean(s^2) + eps) * weight (fp32)
+ *     a_scale_out[m + Mp*kb] = 1 / scale,  A_out[m + Mp*k] = e4m3fn(clamp(y * scale)),  scale as in fp8bs_quantize_rowwise
+ * The norm sees s before it is rounded to residual_out.  X is [rows, K] with a row pitch of ldx elements, residual (may be NULL:
+ * no addition, residual_out is not written) [rows, K] with a pitch of ldr, residual_out [rows, K] without gaps; residual_out may be
+ * the residual itself or X itself if that has no gaps (ldr or ldx = K), and must not overlap them otherwise.  Each of X, residual
+ * and weight [K] is bf16 (its flag != 0) or fp32.  Any rows >= 1: Mp is rows rounded up to a multiple of 16, and the rows behind
+ * the last are written as zeros (scale fp8_max / 1e-12), so that one token is an operand of 16 rows.  A row that holds a NaN or an
+ * infinity gets NaN bytes and scales where torch's arithmetic has NaN.  K a multiple of 128 (rows of more
+ * than 16384 columns, in fp32 with an fp32 residual than 13312, are read twice); all pointers but a_scale_out 16-byte aligned,
+ * and the pitches multiples of 16 bytes; 0 < fp8_max <= 448; eps >= 0.  Asynchronous on `stream`. */
+int fp8bs_rmsnorm_quantize(const void* X, int x_is_bf16, long long ldx, const void* residual, int r_is_bf16, long long ldr,
+                           void* residual_out, const void* weight, int w_is_bf16, void* A_out, float* a_scale_out, int rows,
+                           int K, float eps, float fp8_max, void* stream);
+
 /* Seeded synthetic inputs (role of genMat, utils.h:25-33, but counter-based so that any
  * slice can be generated independently).  Elements: N(0,1) rounded to nearest-even e4m3fn,
  * clamped to |x| <= 240, |x| < 2^-6 flushed to +0 -- every value exists in e4m3fnuz too.
