@@ -1628,7 +1628,6 @@ int fp8bs_rmsnorm_quantize(const void* X, int x_is_bf16, long long ldx, const vo
     p.cluster = 0;
     p.w_is_bf16 = w_is_bf16;
     p.eps = eps; p.fp8_max = fp8_max;
-    p.clamp = host_e4m3fn_to_float(float_to_e4m3fn_rne(fp8_max)) != fp8_max;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     using bf16 = __nv_bfloat16;
     if (!residual) return x_is_bf16 ? launch_rmsnorm<bf16, void>(p, dev, st) : launch_rmsnorm<float, void>(p, dev, st);

@@ -42,7 +42,6 @@ struct NormParams {
     int rows, M, K;                    // M: rows rounded up to 16
     int cluster;
     int w_is_bf16;
-    int clamp;                         // fp8_max is no e4m3 value: a product that rounding has put above it would not round back
     float eps, fp8_max;
 };
 
@@ -53,13 +52,6 @@ __device__ __forceinline__ float max_nan(float a, float b)
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
-__device__ __forceinline__ float min_nan(float a, float b)
-{
-    float d;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
 // Reduces 16 values per lane, one per row, over the 32 lanes: the halving butterfly of quantize.cuh (16 shuffles).  Lanes 2 r
 // and 2 r + 1 return row r's.
 template <class Op>
@@ -136,19 +128,32 @@ struct Quad<__nv_bfloat16> {
     }
 };
 
-// s = x + r of a 16 x 128 block, from shared memory (a CTA's rows, `width` columns each) or from global memory; rows behind the
-// last are 0.
+// s = x + r of 16 rows and four columns.  From shared memory, where the rows behind the last hold zeros ...
 template <class X, class R>
-__device__ __forceinline__ void norm_read(const NormParams& p, bool shared, const uint8_t* xs, const uint8_t* rs, int width, int col,
-                                          int r0, int k, f32x2 (&s)[16][2])
+__device__ __forceinline__ void norm_read_shared(const uint8_t* xs, const uint8_t* rs, int width, int col, f32x2 (&s)[16][2])
+{
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        Quad<X> x;
+        x.from_shared(xs + (i * width + col) * static_cast<int>(sizeof(X)));
+        s[i][0] = x.pair(0);
+        s[i][1] = x.pair(1);
+        if constexpr (!std::is_void<R>::value) {
+            Quad<R> r;
+            r.from_shared(rs + (i * width + col) * static_cast<int>(sizeof(R)));
+            s[i][0] = add_f32x2(s[i][0], r.pair(0));
+            s[i][1] = add_f32x2(s[i][1], r.pair(1));
+        }
+    }
+}
+// ... and from global memory.
+template <class X, class R>
+__device__ __forceinline__ void norm_read(const NormParams& p, int r0, int k, f32x2 (&s)[16][2])
 {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         Quad<X> x{};
-        if (r0 + i < p.rows) {
-            if (shared) x.from_shared(xs + (i * width + col) * static_cast<int>(sizeof(X)));
-            else x.from_global(p.x, (r0 + i) * p.ldx + k);
-        }
+        if (r0 + i < p.rows) x.from_global(p.x, (r0 + i) * p.ldx + k);
         s[i][0] = x.pair(0);
         s[i][1] = x.pair(1);
     }
@@ -156,10 +161,7 @@ __device__ __forceinline__ void norm_read(const NormParams& p, bool shared, cons
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             Quad<R> r{};
-            if (r0 + i < p.rows) {
-                if (shared) r.from_shared(rs + (i * width + col) * static_cast<int>(sizeof(R)));
-                else r.from_global(p.r, (r0 + i) * p.ldr + k);
-            }
+            if (r0 + i < p.rows) r.from_global(p.r, (r0 + i) * p.ldr + k);
             s[i][0] = add_f32x2(s[i][0], r.pair(0));
             s[i][1] = add_f32x2(s[i][1], r.pair(1));
         }
@@ -172,29 +174,32 @@ __device__ __forceinline__ float sum_of_squares(f32x2 a, f32x2 b)
     return f32x2_lo(q) + f32x2_hi(q);
 }
 
-// s -> r_out; s = s * w; returns the largest |s * w| of the block in row lane / 2.
-template <class R>
-__device__ __forceinline__ float norm_weigh(const NormParams& p, int r0, int k, int lane, f32x2 (&s)[16][2])
+__device__ __forceinline__ void norm_weights(const NormParams& p, int k, f32x2 (&w)[2])
 {
-    f32x2 w0, w1;
     if (p.w_is_bf16) {
         Quad<__nv_bfloat16> q;
         q.v = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.w) + k));
-        w0 = q.pair(0);
-        w1 = q.pair(1);
+        w[0] = q.pair(0);
+        w[1] = q.pair(1);
     } else {
         Quad<float> q;
         q.v = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(p.w) + k));
-        w0 = q.pair(0);
-        w1 = q.pair(1);
+        w[0] = q.pair(0);
+        w[1] = q.pair(1);
     }
+}
+
+// s -> r_out; s = s * w; returns the largest |s * w| of the block in row lane / 2.
+template <class R>
+__device__ __forceinline__ float norm_weigh(const NormParams& p, int r0, int k, int lane, const f32x2 (&w)[2], f32x2 (&s)[16][2])
+{
     float amax[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         if constexpr (!std::is_void<R>::value)
             if (r0 + i < p.rows) Quad<R>::store(p.r_out, static_cast<long long>(r0 + i) * p.K + k, s[i][0], s[i][1]);
-        s[i][0] = mul_f32x2(s[i][0], w0);
-        s[i][1] = mul_f32x2(s[i][1], w1);
+        s[i][0] = mul_f32x2(s[i][0], w[0]);
+        s[i][1] = mul_f32x2(s[i][1], w[1]);
         amax[i] = max_nan(max_nan(fabsf(f32x2_lo(s[i][0])), fabsf(f32x2_hi(s[i][0]))),
                           max_nan(fabsf(f32x2_lo(s[i][1])), fabsf(f32x2_hi(s[i][1]))));
     }
@@ -209,7 +214,10 @@ __device__ __forceinline__ void norm_store(const NormParams& p, int r0, int kb, 
     const float m = max_nan(__fmul_rn(amax, rs), 1e-12f);
     const float sc = __fmul_rn(__fdiv_rn(1.0f, m), p.fp8_max);                       // as in quantize.cuh
     if ((lane & 1) == 0) p.scale_out[static_cast<size_t>(kb) * p.M + r0 + (lane >> 1)] = __fdiv_rn(1.0f, sc);
-    const float mine = __fmul_rn(rs, sc);
+    // No product below may round to more than fp8_max: the factor is five roundings off at most, and eight are taken off where the
+    // largest product shows one.
+    float mine = __fmul_rn(rs, sc);
+    if (__fmul_rn(amax, mine) > p.fp8_max) mine = __fmul_rn(mine, 1.0f - 0x1p-21f);
     uint8_t* dst = p.out + static_cast<size_t>(kb * 128 + lane * 4) * p.M + r0;
     uint32_t q[4][4];                                                                // [column][four rows]
 #pragma unroll
@@ -220,9 +228,6 @@ __device__ __forceinline__ void norm_store(const NormParams& p, int r0, int kb, 
             const float f = __shfl_sync(0xffffffffu, mine, 2 * (4 * g + i));
             const f32x2 ff = pack_f32x2(f, f), a = mul_f32x2(t[4 * g + i][0], ff), b = mul_f32x2(t[4 * g + i][1], ff);
             v[i][0] = f32x2_lo(a); v[i][1] = f32x2_hi(a); v[i][2] = f32x2_lo(b); v[i][3] = f32x2_hi(b);
-            if (p.clamp)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[i][j] = min_nan(max_nan(v[i][j], -p.fp8_max), p.fp8_max);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) q[j][g] = cvt_e4m3x2(v[0][j], v[1][j]) | (cvt_e4m3x2(v[2][j], v[3][j]) << 16);
@@ -261,6 +266,14 @@ rmsnorm_quantize_kernel(const NormParams p)
     // 16 rows of x and of r, a copy per row, by warp 0
     auto request = [&](int g) {
         const int rows = min(NORM_ROWS, p.rows - g * NORM_ROWS);
+        if (rows < NORM_ROWS) {                      // the last 16 rows: zeros behind the last
+            for (uint32_t i = static_cast<uint32_t>(rows * width) * sizeof(X) + lane * 16; i < NORM_ROWS * width * sizeof(X); i += 512)
+                *reinterpret_cast<uint4*>(xs + i) = make_uint4(0u, 0u, 0u, 0u);
+            if (ADD)
+                for (uint32_t i = static_cast<uint32_t>(rows * width) * sizeof(RT) + lane * 16; i < NORM_ROWS * width * sizeof(RT); i += 512)
+                    *reinterpret_cast<uint4*>(rs + i) = make_uint4(0u, 0u, 0u, 0u);
+            __syncwarp();
+        }
         if (lane == 0) ptx::mbar_arrive_expect_tx(rows_bar, static_cast<uint32_t>(rows * cols * (sizeof(X) + (ADD ? sizeof(RT) : 0))));
         __syncwarp();
         const long long row = g * NORM_ROWS + (lane & 15), col = rank * width;
@@ -287,8 +300,18 @@ rmsnorm_quantize_kernel(const NormParams p)
     if (warp == 0) request(static_cast<int>(blockIdx.x) / C);          // grid <= C * groups
     if (C > 1) ptx::cluster_wait();
 
+    auto cta_sum = [&](const float* ws, int row) {
+        float v[NORM_MOST_WARPS], sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NORM_MOST_WARPS; ++j) v[j] = j < warps ? ws[j * NORM_ROWS + row] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < NORM_MOST_WARPS; ++j) sum += v[j];
+        return sum;
+    };
     const bool mine = kb < KB;
     const int k = kb * 128 + lane * 4, col = warp * 128 + lane * 4;
+    f32x2 w[2] = {0ull, 0ull};
+    if (mine) norm_weights(p, k, w);
     bool ok = true;
     uint32_t n = 0;
     for (int g = static_cast<int>(blockIdx.x) / C; g < groups; g += step, ++n) {
@@ -297,7 +320,7 @@ rmsnorm_quantize_kernel(const NormParams p)
         ok = ok && wait_bounded(rows_bar, odd, abort_flag, p.status, DS_TIMEOUT_STAGE_FULL);
         f32x2 t[16][2];
         float part[16];
-        if (mine) norm_read<X, R>(p, true, xs, rs, width, col, r0, k, t);
+        if (mine) norm_read_shared<X, R>(xs, rs, width, col, t);
 #pragma unroll
         for (int i = 0; i < 16; ++i) part[i] = mine ? sum_of_squares(t[i][0], t[i][1]) : 0.0f;
         const float sum = reduce_16_rows(part, lane, [](float a, float b) { return a + b; });
@@ -315,20 +338,22 @@ rmsnorm_quantize_kernel(const NormParams p)
             for (int i = static_cast<int>(threadIdx.x); i < NORM_ROWS * C; i += static_cast<int>(blockDim.x)) {
                 const int row = i % NORM_ROWS;
                 const uint32_t peer = static_cast<uint32_t>(i / NORM_ROWS);
-                float mine_ = 0.0f;
-                for (int j = 0; j < warps; ++j) mine_ += ws[j * NORM_ROWS + row];
-                ptx::st_async_f32(ptx::mapa(ptx::smem_u32(cta_sums + (odd * NORM_MAX_CLUSTER + rank) * NORM_ROWS + row), peer), mine_,
+                ptx::st_async_f32(ptx::mapa(ptx::smem_u32(cta_sums + (odd * NORM_MAX_CLUSTER + rank) * NORM_ROWS + row), peer), cta_sum(ws, row),
                                   ptx::mapa(bar, peer));
             }
         } else {
-            for (int j = 0; j < warps; ++j) total += ws[j * NORM_ROWS + (lane >> 1)];
+            total = cta_sum(ws, lane >> 1);
         }
         float amax = 0.0f;
-        if (mine) amax = norm_weigh<R>(p, r0, k, lane, t);
+        if (mine) amax = norm_weigh<R>(p, r0, k, lane, w, t);
         if (C > 1) {
             ok = wait_bounded(sums_bar + 8u * odd, (n >> 1) & 1u, abort_flag, p.status, DS_TIMEOUT_PEER_PARTIAL);
             ok = __all_sync(0xffffffffu, ok);
-            for (int c = 0; c < C; ++c) total += cta_sums[(odd * NORM_MAX_CLUSTER + c) * NORM_ROWS + (lane >> 1)];
+            float v[NORM_MAX_CLUSTER];
+#pragma unroll
+            for (int c = 0; c < NORM_MAX_CLUSTER; ++c) v[c] = c < C ? cta_sums[(odd * NORM_MAX_CLUSTER + c) * NORM_ROWS + (lane >> 1)] : 0.0f;
+#pragma unroll
+            for (int c = 0; c < NORM_MAX_CLUSTER; ++c) total += v[c];
         }
         if (mine && ok) norm_store(p, r0, kb, lane, t, norm_rstd(p, total), amax);
     }
@@ -361,7 +386,7 @@ rmsnorm_quantize_long_kernel(const NormParams p)
 #pragma unroll
     for (int i = 0; i < 16; ++i) part[i] = 0.0f;
     for (int kb = kb0; kb < KB; kb += STEP) {
-        norm_read<X, R>(p, false, nullptr, nullptr, 0, 0, r0, kb * 128 + lane * 4, t);
+        norm_read<X, R>(p, r0, kb * 128 + lane * 4, t);
 #pragma unroll
         for (int i = 0; i < 16; ++i) part[i] += sum_of_squares(t[i][0], t[i][1]);
     }
@@ -383,8 +408,10 @@ rmsnorm_quantize_long_kernel(const NormParams p)
     const float rstd = norm_rstd(p, total);
     for (int kb = kb0; kb < KB; kb += STEP) {
         const int k = kb * 128 + lane * 4;
-        norm_read<X, R>(p, false, nullptr, nullptr, 0, 0, r0, k, t);
-        const float amax = norm_weigh<R>(p, r0, k, lane, t);
+        norm_read<X, R>(p, r0, k, t);
+        f32x2 w[2];
+        norm_weights(p, k, w);
+        const float amax = norm_weigh<R>(p, r0, k, lane, w, t);
         norm_store(p, r0, kb, lane, t, rstd, amax);
     }
 }
