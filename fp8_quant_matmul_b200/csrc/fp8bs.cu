@@ -649,11 +649,13 @@ static int norm_clusters(int device, int cluster, int warps, int smem, int* out)
 template <class X, class R>
 static int launch_rmsnorm(NormParams p, const DeviceInfo* dev, cudaStream_t st)
 {
-    // As few CTAs per cluster as hold the row, and as few warps in each (K = 2304: 3 x 6 instead of 3 x 8).
-    const int KB = p.K / 128, groups = p.M / NORM_ROWS;
-    const int cluster = std::min(ceil_div(KB, NORM_WARPS), NORM_MAX_CLUSTER), warps = ceil_div(KB, cluster);
     int element = sizeof(X);
     if constexpr (!std::is_void<R>::value) element += sizeof(R);
+    // As few CTAs per cluster as hold the row, and as few warps in each (K = 2304: 3 x 6 instead of 3 x 8).  Eight bytes per column
+    // (fp32 twice): six warps, whose buffers leave room for a second CTA.
+    const int KB = p.K / 128, groups = p.M / NORM_ROWS;
+    const int warps = ceil_div(KB, std::min(ceil_div(KB, element == 8 ? 6 : NORM_WARPS), NORM_MAX_CLUSTER));
+    const int cluster = std::min(ceil_div(KB, warps), NORM_MAX_CLUSTER);         // every CTA has a block at least
     const long long buffers = static_cast<long long>(NORM_ROWS) * 128 * warps * element;
     if (warps > NORM_MOST_WARPS || buffers > NORM_SMEM_LIMIT)
         return launch_grid(rmsnorm_quantize_long_kernel<X, R>, dim3(static_cast<unsigned>(groups * NORM_MAX_CLUSTER), 1, 1), NORM_MAX_CLUSTER,
@@ -1627,6 +1629,7 @@ int fp8bs_rmsnorm_quantize(const void* X, int x_is_bf16, long long ldx, const vo
     p.status = dev->status_ptr;
     p.cluster = 0;
     p.w_is_bf16 = w_is_bf16;
+    p.inv_K = 1.0f / static_cast<float>(K);
     p.eps = eps; p.fp8_max = fp8_max;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     using bf16 = __nv_bfloat16;

@@ -10,7 +10,8 @@
 // sums of squares through distributed shared memory (64 bytes from each to each, counted by an mbarrier of the receiver).  All
 // that does not need the norm is done before the exchange: s * w and its largest magnitude per row and block; after it one factor
 // per row and block is left, 1 / rms times the scale.  The 16 rows of a lane's column are 16 neighbouring bytes of A, so the
-// quantised values leave the registers as one 16-byte store per column, without going through shared memory.
+// quantised values leave straight from the registers, two groups of 16 rows (a 32-byte sector) at a time: as 16-byte stores they cost
+// 13 of 48 us on 4096 x 7168 bf16 with residual, this way 4 of 39.
 // The clusters are persistent and their rows arrive by bulk copies: a CTA's buffer is requested anew as soon as its warps have it in
 // registers, so that the next 16 rows are on their way while these are reduced, exchanged and stored.
 // Sums are added in a fixed order (lanes, warps, CTAs).
@@ -42,7 +43,7 @@ struct NormParams {
     int rows, M, K;                    // M: rows rounded up to 16
     int cluster;
     int w_is_bf16;
-    float eps, fp8_max;
+    float inv_K, eps, fp8_max;
 };
 
 // torch's maximum: NaN if either is (fmaxf drops it), so that a NaN in a row shows in its bytes and scales.
@@ -52,31 +53,38 @@ __device__ __forceinline__ float max_nan(float a, float b)
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
-// Reduces 16 values per lane, one per row, over the 32 lanes: the halving butterfly of quantize.cuh (16 shuffles).  Lanes 2 r
-// and 2 r + 1 return row r's.
-template <class Op>
-__device__ __forceinline__ float reduce_16_rows(const float (&a)[16], int lane, Op op)
+// The largest magnitude over a warp's lanes, NaN if one is.
+__device__ __forceinline__ float warp_absmax_nan(float a)
+{
+    float d;
+    asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(a));
+    return d;
+}
+
+// Adds up 16 values per lane, one per row, over the 32 lanes: the halving butterfly of quantize.cuh (16 shuffles).  Lanes 2 r and
+// 2 r + 1 return row r's.
+__device__ __forceinline__ float sum_16_rows(const float (&a)[16], int lane)
 {
     const bool b4 = (lane & 16) != 0, b3 = (lane & 8) != 0, b2 = (lane & 4) != 0, b1 = (lane & 2) != 0;
     float h8[8], h4[4], h2[2];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float give = b4 ? a[j] : a[j + 8], keep = b4 ? a[j + 8] : a[j];
-        h8[j] = op(keep, __shfl_xor_sync(0xffffffffu, give, 16));
+        h8[j] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const float give = b3 ? h8[j] : h8[j + 4], keep = b3 ? h8[j + 4] : h8[j];
-        h4[j] = op(keep, __shfl_xor_sync(0xffffffffu, give, 8));
+        h4[j] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const float give = b2 ? h4[j] : h4[j + 2], keep = b2 ? h4[j + 2] : h4[j];
-        h2[j] = op(keep, __shfl_xor_sync(0xffffffffu, give, 4));
+        h2[j] = keep + __shfl_xor_sync(0xffffffffu, give, 4);
     }
     const float give = b1 ? h2[0] : h2[1], keep = b1 ? h2[1] : h2[0];
-    const float one = op(keep, __shfl_xor_sync(0xffffffffu, give, 2));
-    return op(one, __shfl_xor_sync(0xffffffffu, one, 1));
+    const float one = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+    return one + __shfl_xor_sync(0xffffffffu, one, 1);
 }
 
 typedef unsigned long long f32x2;      // two fp32 values, the operand of the packed instructions
@@ -189,57 +197,80 @@ __device__ __forceinline__ void norm_weights(const NormParams& p, int k, f32x2 (
     }
 }
 
-// s -> r_out; s = s * w; returns the largest |s * w| of the block in row lane / 2.
+// s -> r_out (`rows` of the 16); s = s * w; returns the largest |s * w| of the block in row lane / 2.
 template <class R>
 __device__ __forceinline__ float norm_weigh(const NormParams& p, int r0, int k, int lane, const f32x2 (&w)[2], f32x2 (&s)[16][2])
 {
-    float amax[16];
+    if constexpr (!std::is_void<R>::value) {
+        const long long at = static_cast<long long>(r0) * p.K + k;
+        const int rows = p.rows - r0;
+        if (rows >= NORM_ROWS) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) Quad<R>::store(p.r_out, at + static_cast<long long>(i) * p.K, s[i][0], s[i][1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i < rows) Quad<R>::store(p.r_out, at + static_cast<long long>(i) * p.K, s[i][0], s[i][1]);
+        }
+    }
+    float mine = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        if constexpr (!std::is_void<R>::value)
-            if (r0 + i < p.rows) Quad<R>::store(p.r_out, static_cast<long long>(r0 + i) * p.K + k, s[i][0], s[i][1]);
         s[i][0] = mul_f32x2(s[i][0], w[0]);
         s[i][1] = mul_f32x2(s[i][1], w[1]);
-        amax[i] = max_nan(max_nan(fabsf(f32x2_lo(s[i][0])), fabsf(f32x2_hi(s[i][0]))),
-                          max_nan(fabsf(f32x2_lo(s[i][1])), fabsf(f32x2_hi(s[i][1]))));
+        const float m = warp_absmax_nan(max_nan(max_nan(fabsf(f32x2_lo(s[i][0])), fabsf(f32x2_hi(s[i][0]))),
+                                                max_nan(fabsf(f32x2_lo(s[i][1])), fabsf(f32x2_hi(s[i][1])))));
+        if ((lane >> 1) == i) mine = m;
     }
-    return reduce_16_rows(amax, lane, [](float a, float b) { return max_nan(a, b); });
+    return mine;
 }
 
-// The bytes and scales of one 16 x 128 block from t = s * w.  rstd, amax: 1 / rms and the largest |t| of row lane / 2.
-__device__ __forceinline__ void norm_store(const NormParams& p, int r0, int kb, int lane, const f32x2 (&t)[16][2], float rstd, float amax)
+// What t = s * w is multiplied with in row lane / 2 of a 16 x 128 block before it is rounded to 8 bits; stores the inverse scale.
+// rstd, amax: 1 / rms and the largest |t| of that row.
+__device__ __forceinline__ float norm_factor(const NormParams& p, int r0, int kb, int lane, float rstd, float amax)
 {
     // the rows behind the last are zeros whatever eps is
     const float rs = r0 + (lane >> 1) < p.rows ? rstd : 0.0f;
     const float m = max_nan(__fmul_rn(amax, rs), 1e-12f);
-    const float sc = __fmul_rn(__fdiv_rn(1.0f, m), p.fp8_max);                       // as in quantize.cuh
-    if ((lane & 1) == 0) p.scale_out[static_cast<size_t>(kb) * p.M + r0 + (lane >> 1)] = __fdiv_rn(1.0f, sc);
-    // No product below may round to more than fp8_max: the factor is five roundings off at most, and eight are taken off where the
+    const float sc = __fmul_rn(__frcp_rn(m), p.fp8_max);                             // as in quantize.cuh
+    if ((lane & 1) == 0) p.scale_out[static_cast<size_t>(kb) * p.M + r0 + (lane >> 1)] = __frcp_rn(sc);
+    // No product may round to more than fp8_max: the factor is five roundings off at most, and eight are taken off where the
     // largest product shows one.
-    float mine = __fmul_rn(rs, sc);
-    if (__fmul_rn(amax, mine) > p.fp8_max) mine = __fmul_rn(mine, 1.0f - 0x1p-21f);
-    uint8_t* dst = p.out + static_cast<size_t>(kb * 128 + lane * 4) * p.M + r0;
-    uint32_t q[4][4];                                                                // [column][four rows]
+    const float f = __fmul_rn(rs, sc);
+    return __fmul_rn(amax, f) > p.fp8_max ? __fmul_rn(f, 1.0f - 0x1p-21f) : f;
+}
+// t = t * factor
+__device__ __forceinline__ void norm_scale(float factor, f32x2 (&t)[16][2])
+{
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        float v[4][4];                                                               // [row][column]
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float f = __shfl_sync(0xffffffffu, mine, 2 * (4 * g + i));
-            const f32x2 ff = pack_f32x2(f, f), a = mul_f32x2(t[4 * g + i][0], ff), b = mul_f32x2(t[4 * g + i][1], ff);
-            v[i][0] = f32x2_lo(a); v[i][1] = f32x2_hi(a); v[i][2] = f32x2_lo(b); v[i][3] = f32x2_hi(b);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) q[j][g] = cvt_e4m3x2(v[0][j], v[1][j]) | (cvt_e4m3x2(v[2][j], v[3][j]) << 16);
+    for (int i = 0; i < 16; ++i) {
+        const float f = __shfl_sync(0xffffffffu, factor, 2 * i);
+        t[i][0] = mul_f32x2(t[i][0], pack_f32x2(f, f));
+        t[i][1] = mul_f32x2(t[i][1], pack_f32x2(f, f));
     }
+}
+// The bytes of column j of a lane's four, 16 rows.
+__device__ __forceinline__ void norm_bytes(const f32x2 (&t)[16][2], int j, uint32_t (&q)[4])
+{
+    auto v = [&](int i) { return (j & 1) ? f32x2_hi(t[i][j >> 1]) : f32x2_lo(t[i][j >> 1]); };
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<uint4*>(dst + static_cast<size_t>(j) * p.M) = make_uint4(q[j][0], q[j][1], q[j][2], q[j][3]);
+    for (int g = 0; g < 4; ++g) q[g] = cvt_e4m3x2(v(4 * g), v(4 * g + 1)) | (cvt_e4m3x2(v(4 * g + 2), v(4 * g + 3)) << 16);
+}
+
+__device__ __forceinline__ void store_16(uint8_t* dst, const uint32_t (&q)[4])
+{
+    *reinterpret_cast<uint4*>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
+}
+__device__ __forceinline__ void store_32(uint8_t* dst, const uint32_t (&a)[4], const uint32_t (&b)[4])
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(__cvta_generic_to_global(dst)), "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3])
+                 : "memory");
 }
 
 __device__ __forceinline__ float norm_rstd(const NormParams& p, float total)
 {
-    return __frsqrt_rn(__fadd_rn(__fdiv_rn(total, static_cast<float>(p.K)), p.eps));
+    return __frsqrt_rn(__fadd_rn(__fmul_rn(total, p.inv_K), p.eps));
 }
 
 // Rows that a cluster holds.  grid = a multiple of the cluster size, 32 threads per block of a CTA's share.
@@ -262,7 +293,10 @@ rmsnorm_quantize_kernel(const NormParams p)
     const uint32_t rows_bar = ptx::smem_u32(bars), sums_bar = rows_bar + 8;
     volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(bars + 3);
 
-    const int groups = p.M / NORM_ROWS, step = static_cast<int>(gridDim.x) / C;
+    // the groups of 16 rows that this cluster does, one after the other
+    const int groups = p.M / NORM_ROWS, clusters = static_cast<int>(gridDim.x) / C, id = static_cast<int>(blockIdx.x) / C;
+    const int g0 = static_cast<int>(static_cast<long long>(groups) * id / clusters);
+    const int g1 = static_cast<int>(static_cast<long long>(groups) * (id + 1) / clusters);
     // 16 rows of x and of r, a copy per row, by warp 0
     auto request = [&](int g) {
         const int rows = min(NORM_ROWS, p.rows - g * NORM_ROWS);
@@ -297,15 +331,18 @@ rmsnorm_quantize_kernel(const NormParams p)
     if (C > 1) ptx::cluster_arrive();                // waited for before anything is sent to a peer: its barriers exist
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    if (warp == 0) request(static_cast<int>(blockIdx.x) / C);          // grid <= C * groups
+    if (warp == 0) request(g0);                      // clusters <= groups
     if (C > 1) ptx::cluster_wait();
 
     auto cta_sum = [&](const float* ws, int row) {
-        float v[NORM_MOST_WARPS], sum = 0.0f;
+        float sum = 0.0f;
+        for (int j0 = 0; j0 < warps; j0 += NORM_WARPS) {
+            float v[NORM_WARPS];
 #pragma unroll
-        for (int j = 0; j < NORM_MOST_WARPS; ++j) v[j] = j < warps ? ws[j * NORM_ROWS + row] : 0.0f;
+            for (int j = 0; j < NORM_WARPS; ++j) v[j] = j0 + j < warps ? ws[(j0 + j) * NORM_ROWS + row] : 0.0f;
 #pragma unroll
-        for (int j = 0; j < NORM_MOST_WARPS; ++j) sum += v[j];
+            for (int j = 0; j < NORM_WARPS; ++j) sum += v[j];
+        }
         return sum;
     };
     const bool mine = kb < KB;
@@ -314,7 +351,12 @@ rmsnorm_quantize_kernel(const NormParams p)
     if (mine) norm_weights(p, k, w);
     bool ok = true;
     uint32_t n = 0;
-    for (int g = static_cast<int>(blockIdx.x) / C; g < groups; g += step, ++n) {
+    // Bytes of a column leave 32 at a time: the first 16 of an aligned 32 wait in registers for the next 16 rows.  Which rows are first
+    // depends on the column where a column is not a multiple of 32 bytes long.
+    uint8_t* const dst = p.out + static_cast<size_t>(k) * p.M;
+    uint32_t held[4][4];
+    const uint32_t start = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(dst) >> 4), long_by = static_cast<uint32_t>(groups);
+    for (int g = g0; g < g1; ++g, ++n) {
         const int r0 = g * NORM_ROWS;
         const uint32_t odd = n & 1u;
         ok = ok && wait_bounded(rows_bar, odd, abort_flag, p.status, DS_TIMEOUT_STAGE_FULL);
@@ -323,14 +365,14 @@ rmsnorm_quantize_kernel(const NormParams p)
         if (mine) norm_read_shared<X, R>(xs, rs, width, col, t);
 #pragma unroll
         for (int i = 0; i < 16; ++i) part[i] = mine ? sum_of_squares(t[i][0], t[i][1]) : 0.0f;
-        const float sum = reduce_16_rows(part, lane, [](float a, float b) { return a + b; });
+        const float sum = sum_16_rows(part, lane);
         float* ws = warp_sums + odd * NORM_MOST_WARPS * NORM_ROWS;
         if ((lane & 1) == 0) ws[warp * NORM_ROWS + (lane >> 1)] = sum;
         // everybody has read the rows, and the sums are there.  A set of sums is written again two rounds later, which the barrier of
         // the round between keeps apart (for the peers': a CTA sends round n + 2 after it has round n + 1 from everybody).
         ok = __syncthreads_and(ok);
         if (!ok) break;
-        if (warp == 0 && g + step < groups) request(g + step);
+        if (warp == 0 && g + 1 < g1) request(g + 1);
         float total = 0.0f;
         if (C > 1) {
             const uint32_t bar = sums_bar + 8u * odd;
@@ -355,7 +397,31 @@ rmsnorm_quantize_kernel(const NormParams p)
 #pragma unroll
             for (int c = 0; c < NORM_MAX_CLUSTER; ++c) total += v[c];
         }
-        if (mine && ok) norm_store(p, r0, kb, lane, t, norm_rstd(p, total), amax);
+        if (mine && ok) {
+            norm_scale(norm_factor(p, r0, kb, lane, norm_rstd(p, total), amax), t);
+            // FIRST bit j: the bytes of column j are the first 16 of an aligned 32
+            auto leave = [&](auto first) {
+                constexpr int FIRST = decltype(first)::value;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint8_t* to = dst + static_cast<size_t>(j) * p.M + r0;
+                    if ((FIRST >> j) & 1) {
+                        norm_bytes(t, j, held[j]);
+                        if (g + 1 == g1) store_16(to, held[j]);
+                    } else {
+                        uint32_t q[4];
+                        norm_bytes(t, j, q);
+                        if (g > g0) store_32(to - 16, held[j], q);
+                        else store_16(to, q);
+                    }
+                }
+            };
+            const uint32_t even = (start + static_cast<uint32_t>(g)) & 1u, next = (even + long_by) & 1u;     // of columns 0, 2 and 1, 3
+            if (even == 0u && next == 0u) leave(std::integral_constant<int, 15>{});
+            else if (even != 0u && next != 0u) leave(std::integral_constant<int, 0>{});
+            else if (even == 0u) leave(std::integral_constant<int, 5>{});
+            else leave(std::integral_constant<int, 10>{});
+        }
     }
     if (!ok) {
         // giving up with copies possibly in flight: a bounded time to land
@@ -390,7 +456,7 @@ rmsnorm_quantize_long_kernel(const NormParams p)
 #pragma unroll
         for (int i = 0; i < 16; ++i) part[i] += sum_of_squares(t[i][0], t[i][1]);
     }
-    const float sum = reduce_16_rows(part, lane, [](float a, float b) { return a + b; });
+    const float sum = sum_16_rows(part, lane);
     if ((lane & 1) == 0) warp_sums[warp][lane >> 1] = sum;
     __syncthreads();
     ptx::cluster_wait();
@@ -412,7 +478,13 @@ rmsnorm_quantize_long_kernel(const NormParams p)
         f32x2 w[2];
         norm_weights(p, k, w);
         const float amax = norm_weigh<R>(p, r0, k, lane, w, t);
-        norm_store(p, r0, kb, lane, t, rstd, amax);
+        norm_scale(norm_factor(p, r0, kb, lane, rstd, amax), t);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t q[4];
+            norm_bytes(t, j, q);
+            store_16(p.out + static_cast<size_t>(k + j) * p.M + r0, q);
+        }
     }
 }
 

@@ -2,9 +2,9 @@
 
 Tolerances, before any run.  s = x + r is one rounding of fp32, y = s * rstd * w three more on top of the error of rstd, half that
 of the mean of squares: a square, sums over a lane's 4 columns, 32 lanes, 16 warps one after the other, 8 CTAs one after the other,
-and one more addition per 8192 columns where a warp walks several blocks, the mean and eps: 1 + 2 + 5 + 16 + 8 + 2 + 2 = 36, 18 after
+and one more addition per 8192 columns where a warp walks several blocks, the mean and eps: 1 + 2 + 5 + 16 + 8 + 2 + 3 = 37, 18.5 after
 the root, which adds one.  The product with w, with rstd, the reciprocal, the scale and the inverse scale add one each: 24 roundings
-of 2^-24 and the one of s bound the scales (SCALE_TOL: 26).  A byte is the value times scale, with three more, rounded to e4m3 once: at most half a step (2^-4 of the value's binade, 2^-10 below 2^-6) from the exact product,
+of 2^-24 and the one of s bound the scales (SCALE_TOL: 26, counted up).  A byte is the value times scale, with three more, rounded to e4m3 once: at most half a step (2^-4 of the value's binade, 2^-10 below 2^-6) from the exact product,
 and those 32 roundings (VALUE_TOL) of its value."""
 import itertools
 
@@ -54,7 +54,7 @@ def check_sum(out, s):
     assert ((out.double() - s).abs() <= s.abs() * torch.finfo(out.dtype).eps / 2 * (1 + 2.0 ** -12) + 2.0 ** -24 * s.abs()).all()
 
 
-SHAPES = [(1, 128), (1, 7168), (3, 384), (15, 1024), (16, 1152), (17, 2304), (40, 512), (333, 896), (64, 8192), (5, 8320), (18, 14336), (18, 16384), (33, 20480)]
+SHAPES = [(1, 128), (1, 7168), (3, 384), (15, 1024), (16, 1152), (17, 2304), (40, 512), (333, 896), (2049, 1664), (7, 6272), (64, 8192), (5, 8320), (18, 14336), (18, 16384), (33, 20480)]
 
 
 @pytest.mark.parametrize("rows,K", SHAPES)
