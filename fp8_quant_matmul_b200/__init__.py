@@ -22,6 +22,9 @@ from .api import (  # noqa: F401
     gemm_ref,
     gemm_mn_small_static,
     gemm_scatter,
+    gemm_bias_act,
+    gemm_gated,
+    ACTIVATIONS,
     STATIC_SCRATCH_BYTES,
     gemmGPU,
     quantize_rowwise,

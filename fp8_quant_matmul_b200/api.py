@@ -18,6 +18,7 @@ TILE_PAIR = 0x1000      # tile_n = 256 | TILE_PAIR: a 256 x 256 tile owned by a 
 SPLIT_WORKSPACE = 0x2000  # OR into tile_n: reduce split-K partial sums through the workspace, not in a cluster
 STREAM_K = 0x4000         # OR into tile_n: deal the K blocks of all tiles out evenly over the SMs (needs the workspace)
 SMALL_M = 0x10000         # tile_n = SMALL_M: M <= 64, the kernel for few rows (select_path reports 128 | SMALL_M)
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 SHORT_K = 0x8000          # OR into tile_n (0 or 256): K <= 256, both K blocks of a tile stay in tensor memory
 
 # The 18 benchmark shapes (M, N, K) of the reference's results table (README.md:15-25).
@@ -42,6 +43,9 @@ _SIGS = {
     "fp8bs_gemm_mn_small_static": (_c.c_int, [_c.c_void_p] * 5 + [_c.c_int] * 4 + [_c.c_void_p]),
     "fp8bs_gemm_ex": (_c.c_int, [_c.c_void_p] * 5 + [_c.c_int] * 8 + [_c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "fp8bs_gemm_scatter": (_c.c_int, [_c.c_void_p] * 4 + [_c.POINTER(_c.c_void_p)] + [_c.c_int] * 6 + [_c.c_void_p]),
+    "fp8bs_gemm_bias_act": (_c.c_int, [_c.c_void_p] * 5 + [_c.c_int] * 4 + [_c.c_void_p, _c.c_int, _c.c_int, _c.c_void_p, _c.c_longlong,
+                                                                       _c.c_int, _c.c_int, _c.c_void_p]),
+    "fp8bs_gemm_gated": (_c.c_int, [_c.c_void_p] * 8 + [_c.c_int] * 5 + [_c.c_float, _c.c_int, _c.c_int, _c.c_void_p]),
     "fp8bs_gemm_ref": (_c.c_int, [_c.c_void_p] * 5 + [_c.c_int] * 3 + [_c.c_void_p]),
     "fp8bs_select_path": (_c.c_int, [_c.c_int] * 3 + [_c.POINTER(_c.c_int)] * 2),
     "fp8bs_select_path_sms": (_c.c_int, [_c.c_int] * 4 + [_c.POINTER(_c.c_int)] * 3),
@@ -328,6 +332,98 @@ def gemm(A, B, a_scale, b_scale, C=None, M=None, N=None, K=None, path=PATH_AUTO,
         _check(rc, "fp8bs_gemm_ex")
     _set_up.add(index)
     return C
+
+
+def _check_operands(index, M, N, K, rows, activation, pairs):
+    """What the fused calls check before pointers are handed over; returns the activation's number."""
+    if M is None or N is None or K is None:
+        raise ValueError("M, N, K are required (operands are flat column-major buffers)")
+    if not 1 <= rows <= M:
+        raise ValueError("rows has to be in 1..M")
+    for name, t, n, kind in pairs:
+        if t.get_device() != index or not t.is_contiguous():
+            raise ValueError("%s has to be a contiguous tensor on A's device" % name)
+        if t.numel() < n or t.element_size() != kind:
+            raise ValueError("%s has to hold %d elements of %d bytes" % (name, n, kind))
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError("activation has to be one of " + ", ".join(ACTIVATIONS))
+    return act
+
+
+def _check_out(t, rows, N, dtype, index, name):
+    if tuple(t.shape) != (rows, N) or t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+        raise ValueError("%s has to be a contiguous %s tensor [rows, N] on A's device" % (name, dtype))
+
+
+def gemm_bias_act(A, B, a_scale, b_scale, C=None, M=None, N=None, K=None, bias=None, activation="none", residual=None, rows=None,
+                  splits=0, tile_n=0):
+    """C = act(A @ B^T + bias) + residual on the current CUDA stream, in fp32 until the one rounding to bf16.
+
+    A, B, a_scale, b_scale, M, N, K as in gemm().  bias: [N], fp32 or bf16.  activation: "none", "relu", "silu", "gelu" (erf) or "gelu_tanh".
+    residual: bf16 [rows, N], any row stride of whole 16 bytes; C may be the residual itself.  rows (default M): how many of the M rows
+    exist in C and in the residual, e.g. 1 for one token whose A is padded to 16 rows.  splits / tile_n force a kernel.
+    """
+    torch = _torch()
+    if not A.is_cuda:
+        raise RuntimeError("fp8bs.gemm_bias_act needs CUDA tensors; there is no CPU implementation")
+    index = A.get_device()
+    rows = M if rows is None else rows
+    act = _check_operands(index, M, N, K, rows, activation,
+                          (("A", A, M * K, 1), ("B", B, N * K, 1), ("a_scale", a_scale, M * (K // 128), 4),
+                           ("b_scale", b_scale, -(-N // 128) * (K // 128), 4)) if M is not None and N is not None and K is not None else ())
+    bias_ptr, bias_bf16, r_ptr, ldr = None, 0, None, N
+    if bias is not None:
+        bias_bf16 = _is_bf16(bias.dtype, "bias")
+        if tuple(bias.shape) != (N,) or bias.get_device() != index or not bias.is_contiguous():
+            raise ValueError("bias has to be a contiguous tensor [N] on A's device")
+        bias_ptr = bias.data_ptr()
+    if residual is not None:
+        if (tuple(residual.shape) != (rows, N) or residual.dtype is not torch.bfloat16 or residual.get_device() != index
+                or residual.stride(1) != 1):
+            raise ValueError("residual has to be a bf16 tensor [rows, N] on A's device with contiguous rows")
+        r_ptr = residual.data_ptr()
+        ldr = residual.stride(0) if rows > 1 else N
+    if C is None:
+        C = A.new_empty((rows, N), dtype=torch.bfloat16)
+    else:
+        _check_out(C, rows, N, torch.bfloat16, index, "C")
+    _call("fp8bs_gemm_bias_act", index, A.data_ptr(), B.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), C.data_ptr(), M, N, K, rows,
+          bias_ptr, bias_bf16, act, r_ptr, ldr, splits, tile_n)
+    return C
+
+
+def gemm_gated(A, B_gate, B_up, a_scale, gate_scale, up_scale, M=None, N=None, K=None, activation="silu", quantize=False, fp8_max=448.0,
+               H=None, rows=None, splits=0, tile_n=0):
+    """h = act(A @ B_gate^T) * (A @ B_up^T): both projections of a gated feed-forward layer, its activation and product in one launch.
+
+    B_gate, B_up: N x K column-major as B in gemm(), with their scales.  Returns h in bf16 [rows, N] (in H if given), or with quantize=True in
+    8 bits as the next product's operand, like quantize_rowwise: (bytes [N][M] flat, inverse scales [N / 128][M] flat), all M rows.
+    """
+    torch = _torch()
+    if not A.is_cuda:
+        raise RuntimeError("fp8bs.gemm_gated needs CUDA tensors; there is no CPU implementation")
+    index = A.get_device()
+    rows = M if rows is None else rows
+    known = M is not None and N is not None and K is not None
+    n_scales = -(-N // 128) * (K // 128) if known else 0
+    act = _check_operands(index, M, N, K, rows, activation,
+                          (("A", A, M * K, 1), ("B_gate", B_gate, N * K, 1), ("B_up", B_up, N * K, 1), ("a_scale", a_scale, M * (K // 128), 4),
+                           ("gate_scale", gate_scale, n_scales, 4), ("up_scale", up_scale, n_scales, 4)) if known else ())
+    s_ptr = scales = None
+    if quantize:
+        if H is not None:
+            raise ValueError("H is for the bf16 result")
+        H = A.new_empty(M * N, dtype=torch.uint8)
+        scales = A.new_empty(M * (N // 128), dtype=torch.float32)
+        s_ptr = scales.data_ptr()
+    elif H is None:
+        H = A.new_empty((rows, N), dtype=torch.bfloat16)
+    else:
+        _check_out(H, rows, N, torch.bfloat16, index, "H")
+    _call("fp8bs_gemm_gated", index, A.data_ptr(), B_gate.data_ptr(), B_up.data_ptr(), a_scale.data_ptr(), gate_scale.data_ptr(),
+          up_scale.data_ptr(), H.data_ptr(), s_ptr, M, N, K, rows, act, fp8_max, splits, tile_n)
+    return (H, scales) if quantize else H
 
 
 def gemm_scatter(A, B, a_scale, b_scale, dests, M, N, K, n0, n_total, stream=None):

@@ -1,0 +1,137 @@
+// What a fused epilogue does with a finished sum: bias, activation, residual, the gate, all in fp32.
+//   none   x                     silu       x / (1 + exp(-x))
+//   relu   x < 0 ? 0 : x         gelu       x (1 + erf(x / sqrt 2)) / 2
+//                                gelu_tanh  x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) / 2 = x / (1 + exp(-2 sqrt(2/pi) (x + 0.044715 x^3)))
+// silu and gelu_tanh are one function with two constants, x / (1 + 2^(x (a + b x^2))): an exponential and a reciprocal of the
+// special-function unit per element.  Their errors (2^-22 each, and the argument's rounding) are below 1 % of a bf16 step where the
+// result is not itself negligible, and an output in 8 bits has its scale from the largest elements, where 2^(..) is next to nothing.
+#pragma once
+#include "ptx.cuh"
+#include <cuda_bf16.h>
+#include <cstdint>
+#include <type_traits>
+
+namespace fp8bs {
+
+// torch's maximum: NaN if either is (fmaxf drops it), so that a NaN in a group shows in its bytes and scale.
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// The largest magnitude over a warp's lanes, NaN if one is.
+__device__ __forceinline__ float warp_absmax_nan(float a)
+{
+    float d;
+    asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(a));
+    return d;
+}
+// Two fp32 -> two e4m3fn bytes (lo in bits 0-7, hi in bits 8-15), round to nearest even.
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi)
+{
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+enum : int { ACT_NONE = 0, ACT_RELU = 1, ACT_LOGISTIC = 2, ACT_ERF = 3 };
+
+struct Epilogue {
+    const void* bias;               // [N], NULL: none
+    const __nv_bfloat16* residual;  // [rows, N] with a pitch of ldr elements, NULL: none; may be C
+    long long ldr;
+    const float* up_scale;          // gated: b_scale of the second matrix (GemmParams::b_scale is the first one's)
+    uint8_t* q_out;                 // gated with an output in 8 bits: [N][M] ...
+    float* scale_out;               // ... and its inverse scales [N / 128][M]
+    int bias_is_bf16;
+    int act;
+    float a, b;                     // ACT_LOGISTIC, log2 e included
+    float fp8_max;
+};
+
+__device__ __forceinline__ float logistic_times(float x, float a, float b)
+{
+    // The square is held finite, so that b = 0 leaves a and not 0 * infinity.
+    const float z = x * fmaf(b, fminf(x * x, 1e30f), a);
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return x * r;
+}
+// x (1 + erf(x / sqrt 2)) / 2 = max(x, 0) - |x| erfc(|x| / sqrt 2) / 2 with erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), t = 1 / (1 + p z): formula
+// 7.1.26 of Abramowitz and Stegun, off by 1.5e-7 at most, that is 7.5e-8 |x| here; and the tail below 0 has no cancellation.  (CUDA's
+// erff in this place cost the K loop of the pair kernel 15 spilled registers.)
+__device__ __forceinline__ float erf_times(float x)
+{
+    const float ax = fminf(fabsf(x), 100.0f);                        // the tail is 0 there; infinity would be 0 * infinity
+    const float z = ax * 0.70710678118654752f;
+    float t, e;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f, z, 1.0f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * z * -1.4426950408889634f));
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    return (x < 0.0f ? 0.0f : x) - 0.5f * ax * poly * e;             // a NaN stays one
+}
+template <int ACT>
+__device__ __forceinline__ float activate(float x, const Epilogue& e)
+{
+    if constexpr (ACT == ACT_RELU) return x < 0.0f ? 0.0f : x;       // a NaN stays one
+    else if constexpr (ACT == ACT_LOGISTIC) return logistic_times(x, e.a, e.b);
+    else if constexpr (ACT == ACT_ERF) return erf_times(x);
+    else return x;
+}
+// f(integral constant of the activation): one branch per call of this, not per element.
+template <class F>
+__device__ __forceinline__ void with_activation(const Epilogue& e, F f)
+{
+    if (e.act == ACT_LOGISTIC) f(std::integral_constant<int, ACT_LOGISTIC>{});
+    else if (e.act == ACT_ERF) f(std::integral_constant<int, ACT_ERF>{});
+    else if (e.act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
+    else f(std::integral_constant<int, ACT_NONE>{});
+}
+
+// bias[n .. n + 3]
+__device__ __forceinline__ float4 bias_4(const Epilogue& e, int n)
+{
+    if (e.bias_is_bf16) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(e.bias) + n));
+        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                           __uint_as_float(w.y & 0xffff0000u));
+    }
+    return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(e.bias) + n));
+}
+__device__ __forceinline__ float bias_1(const Epilogue& e, int n)
+{
+    return e.bias_is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[n]) : __ldg(static_cast<const float*>(e.bias) + n);
+}
+
+// act(v + bias) + residual of four neighbouring columns of row m.
+__device__ __forceinline__ float4 finish_4(float4 v, const Epilogue& e, int m, int n)
+{
+    uint2 r = make_uint2(0u, 0u);
+    if (e.residual) r = *reinterpret_cast<const uint2*>(e.residual + m * e.ldr + n);
+    if (e.bias) {
+        const float4 b = bias_4(e, n);
+        v = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
+    }
+    with_activation(e, [&](auto act) {
+        constexpr int A = decltype(act)::value;
+        v = make_float4(activate<A>(v.x, e), activate<A>(v.y, e), activate<A>(v.z, e), activate<A>(v.w, e));
+    });
+    if (e.residual)
+        v = make_float4(v.x + __uint_as_float(r.x << 16), v.y + __uint_as_float(r.x & 0xffff0000u), v.z + __uint_as_float(r.y << 16),
+                        v.w + __uint_as_float(r.y & 0xffff0000u));
+    return v;
+}
+
+// The factor that takes a group whose largest magnitude is amax to 8 bits, and the inverse scale to be stored (as in
+// quantize.cuh: scale = fp8_max / max(amax, 1e-12)).  No product with the factor rounds to more than fp8_max: it is three roundings
+// off at most, and eight are taken off where the largest product shows one.
+__device__ __forceinline__ float scale_factor(float amax, float fp8_max, float& inverse)
+{
+    const float sc = __fmul_rn(__frcp_rn(max_nan(amax, 1e-12f)), fp8_max);
+    inverse = __frcp_rn(sc);
+    return __fmul_rn(amax, sc) > fp8_max ? __fmul_rn(sc, 1.0f - 0x1p-21f) : sc;
+}
+
+}  // namespace fp8bs

@@ -110,19 +110,35 @@ static const bool g_use_pdl = []() { const char* e = std::getenv("FP8BS_PDL"); r
 static long long* g_prof_buf = nullptr;
 #endif
 
-template <int BN, int CG, int MODE>
+template <int BN, int CG, int MODE, int EPI = EPI_NONE>
 static int prepare_kernel()
 {
-    CUDA_TRY(cudaFuncSetAttribute(gemm_kernel<BN, CG, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  TileCfg<BN, CG>::SMEM_BYTES));
+    CUDA_TRY(cudaFuncSetAttribute(gemm_kernel<BN, CG, MODE, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  TileCfg<BN, CG>::SMEM_BYTES + epi_smem(EPI)));
     return FP8BS_OK;
 }
 
-template <int T>
+template <int T, int EPI = EPI_NONE>
 static int prepare_small_m()
 {
-    CUDA_TRY(cudaFuncSetAttribute(gemm_small_m_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SmallMCfg<T>::SMEM_BYTES));
+    CUDA_TRY(cudaFuncSetAttribute(gemm_small_m_kernel<T, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, SmallMCfg<T, EPI>::SMEM_BYTES));
     return FP8BS_OK;
+}
+
+template <int EPI>
+static int prepare_fused_small_m()
+{
+    int rc;
+    if ((rc = prepare_small_m<16, EPI>()) || (rc = prepare_small_m<32, EPI>())) return rc;
+    return prepare_small_m<64, EPI>();
+}
+
+template <int EPI>
+static int prepare_gated()
+{
+    int rc;
+    if ((rc = prepare_kernel<256, 2, 0, EPI>()) || (rc = prepare_kernel<256, 1, 0, EPI>()) || (rc = prepare_kernel<256, 1, 2, EPI>())) return rc;
+    return prepare_fused_small_m<EPI>();
 }
 
 template <bool BLOCK_SCALE>
@@ -171,7 +187,10 @@ static int device_setup(DeviceInfo** out)
             (rc = prepare_kernel<128, 1, 3>()) || (rc = prepare_kernel<256, 1, 3>()) ||
             (rc = prepare_kernel<256, 1, 4>()) || (rc = prepare_small_m<16>()) ||
             (rc = prepare_small_m<32>()) || (rc = prepare_small_m<64>()) ||
-            (rc = prepare_quantize<false>()) || (rc = prepare_quantize<true>())) {
+            (rc = prepare_quantize<false>()) || (rc = prepare_quantize<true>()) ||
+            (rc = prepare_kernel<128, 1, 0, EPI_BIAS_ACT>()) || (rc = prepare_kernel<256, 2, 0, EPI_BIAS_ACT>()) ||
+            (rc = prepare_kernel<128, 1, 2, EPI_BIAS_ACT>()) || (rc = prepare_kernel<256, 1, 2, EPI_BIAS_ACT>()) ||
+            (rc = prepare_fused_small_m<EPI_BIAS_ACT>()) || (rc = prepare_gated<EPI_GATED>()) || (rc = prepare_gated<EPI_GATED_FP8>())) {
             d.status = rc;
             return rc;
         }
@@ -250,13 +269,14 @@ constexpr int SMALL_M_MAX = 64;
 // 9.5, .., 6.2 with 8; 32 x 4096 x 2048 (32 tiles) 9.9, 7.5, 6.7, 6.2.  Up to four K blocks the reduction costs more than it
 // saves: 16 x 4608 x 256 2.9, 3.6; 32 x 7168 x 512 4.5, 5.1.  With long K (16 K blocks per CTA and more) two CTAs per SM keep
 // more loads in flight: 16 x 7168 x 7168 16.0 with 2 splits, 14.0 with 4.
-static Config small_m_config(const DeviceModel& dm, int N, int K, int splits)
+// ctas_per_sm: 1 for the gated form, whose CTA keeps twice as many weights in flight.
+static Config small_m_config(const DeviceModel& dm, int N, int K, int splits, int ctas_per_sm = 2)
 {
     const int tiles = ceil_div(N, 128), KB = K / 128;
     int s = splits;
     if (s == 0) {
         s = KB <= 4 ? 1 : dm.sm_count / tiles;
-        if (s >= 1 && KB / s >= 16 && 4 * tiles * s <= 7 * dm.sm_count) s *= 2;
+        if (ctas_per_sm > 1 && s >= 1 && KB / s >= 16 && 4 * tiles * s <= 7 * dm.sm_count) s *= 2;
         if (s > MAX_CLUSTER_SPLITS) s = MAX_CLUSTER_SPLITS;
         if (s > KB) s = KB;
         while (s > 1 && dm.max_clusters[s] < 1) --s;
@@ -443,6 +463,38 @@ static Config plan(const DeviceModel& dm, int device, int M, int N, int K, int p
     return e.cfg;
 }
 
+// The configuration of a fused call (gated: two products, N columns of each).  Those of the estimate that are built for it: the full-K
+// kernel on 128-wide (gated: 2 x 128-wide) and pair tiles, the cluster reduction, few rows.  They need no workspace, and what the
+// epilogue adds to a tile hardly differs between them.
+static int choose_fused(const DeviceModel& dm, int M, int N, int K, bool gated, int splits, int tile_n, Config* out)
+{
+    const int KB = K / 128, t = tile_n & ~FP8BS_SMALL_M;
+    if (splits < 0 || splits > MAX_CLUSTER_SPLITS || splits > KB) return FP8BS_ERR_ARG;
+    if (t != 0 && t != 128 && t != 256 && t != (256 | FP8BS_TILE_PAIR)) return FP8BS_ERR_ARG;
+    if ((tile_n & FP8BS_SMALL_M) && (M > SMALL_M_MAX || (t != 0 && t != 128))) return FP8BS_ERR_ARG;
+    if ((tile_n & FP8BS_SMALL_M) || (tile_n == 0 && M <= SMALL_M_MAX)) {
+        *out = small_m_config(dm, N, K, splits, gated ? 1 : 2);
+        return FP8BS_OK;
+    }
+    double best_cost = 1e300;
+    for (int cg = 1; cg <= 2; ++cg)
+        for (int tn = 128; tn <= 256; tn += 128) {
+            if ((cg == 2 || gated) && tn != 256) continue;
+            if (t && t != (tn | (cg == 2 ? FP8BS_TILE_PAIR : 0))) continue;
+            for (int s = 1; s <= MAX_CLUSTER_SPLITS && s <= KB; ++s) {
+                if (splits && s != splits) continue;
+                if (s > 1 && (cg == 2 || dm.max_clusters[s] < 1)) continue;
+                if (s == 1 && cg == 1 && !gated && tn == 256) continue;            // not built
+                const double c = config_cost(dm, M, gated ? 256 * ceil_div(N, 128) : N, K, tn, s, cg, s > 1 ? 2 : 0);
+                if (c < best_cost) {
+                    best_cost = c;
+                    *out = Config{s > 1 ? FP8BS_PATH_MN_SMALL : FP8BS_PATH_MN_LARGE, tn, s, cg, s > 1 ? 2 : 0, 0};
+                }
+            }
+        }
+    return best_cost < 1e300 ? FP8BS_OK : FP8BS_ERR_ARG;
+}
+
 static size_t config_workspace(int M, int N, const Config& c)
 {
     if (c.mode == 3)                                                 // flags + one partial tile per CTA
@@ -532,7 +584,7 @@ static int encode_few_rows_map(CUtensorMap* tm, const void* base, int M, int K, 
 }
 
 // C as a 2-D bf16 tensor {N, M} (row-major M x N); a store box is 64 columns x 32 rows, 128-byte swizzled.
-static int encode_c_map(CUtensorMap* tm, void* base, int M, int N, int ld)
+static int encode_c_map(CUtensorMap* tm, void* base, int M, int N, long long ld)
 {
     // `base` is the first element of the M x N window this call writes; `ld` is the row pitch of the buffer in elements
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(M)};
@@ -599,7 +651,7 @@ static int launch_clusters(Kernel kernel, int ctas, int cluster, int threads, in
     return launch_grid(kernel, dim3(static_cast<unsigned>(ctas), 1, 1), cluster, threads, smem, stream, args...);
 }
 
-template <int BN, int CG, int MODE>
+template <int BN, int CG, int MODE, int EPI = EPI_NONE>
 static int launch(const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t stream)
 {
     using Cfg = TileCfg<BN, CG>;
@@ -607,15 +659,36 @@ static int launch(const TensorMaps& tm, const GemmParams& p, int sm_count, cudaS
     int groups = units < sm_count / CG ? units : sm_count / CG;    // tile walkers: CTAs or CTA pairs
     if (MODE == 2) groups = units;                                  // one CTA per (tile, K range); a cluster per tile
     if (MODE == 3) groups = stream_k_ctas(p.m_tiles * p.n_tiles, p.K / 128, sm_count);
-    return launch_clusters(gemm_kernel<BN, CG, MODE>, groups * CG, MODE == 2 ? p.splits : CG, Cfg::THREADS, Cfg::SMEM_BYTES, stream,
-                           tm.A, tm.B, tm.C, p);
+    return launch_clusters(gemm_kernel<BN, CG, MODE, EPI>, groups * CG, MODE == 2 ? p.splits : CG, Cfg::THREADS,
+                           Cfg::SMEM_BYTES + epi_smem(EPI), stream, tm.A, tm.B, tm.C, p);
 }
 
-template <int T>
+template <int T, int EPI = EPI_NONE>
 static int launch_small_m(const TensorMaps& tm, const GemmParams& p, cudaStream_t stream)
 {
-    using Cfg = SmallMCfg<T>;
-    return launch_clusters(gemm_small_m_kernel<T>, p.n_tiles * p.splits, p.splits, Cfg::THREADS, Cfg::SMEM_BYTES, stream, tm.A, tm.B, p);
+    using Cfg = SmallMCfg<T, EPI>;
+    return launch_clusters(gemm_small_m_kernel<T, EPI>, p.n_tiles * p.splits, p.splits, Cfg::THREADS, Cfg::SMEM_BYTES, stream, tm.A, tm.B,
+                           tm.C.m[MAP_UP], p);
+}
+
+// The fused calls: bias, activation and residual on 128-wide and pair tiles, or in the cluster reduction ...
+static int launch_bias_act(const Config& c, const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t st)
+{
+    if (c.mode == 5)
+        return p.M <= 16 ? launch_small_m<16, EPI_BIAS_ACT>(tm, p, st) : p.M <= 32 ? launch_small_m<32, EPI_BIAS_ACT>(tm, p, st)
+                                                                       : launch_small_m<64, EPI_BIAS_ACT>(tm, p, st);
+    if (c.mode == 2)
+        return c.tile_n == 256 ? launch<256, 1, 2, EPI_BIAS_ACT>(tm, p, sm_count, st) : launch<128, 1, 2, EPI_BIAS_ACT>(tm, p, sm_count, st);
+    return c.cg == 2 ? launch<256, 2, 0, EPI_BIAS_ACT>(tm, p, sm_count, st) : launch<128, 1, 0, EPI_BIAS_ACT>(tm, p, sm_count, st);
+}
+// ... and the gated pair of products, on tiles of 2 x 128 columns.
+template <int EPI>
+static int launch_gated(const Config& c, const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t st)
+{
+    if (c.mode == 5)
+        return p.M <= 16 ? launch_small_m<16, EPI>(tm, p, st) : p.M <= 32 ? launch_small_m<32, EPI>(tm, p, st) : launch_small_m<64, EPI>(tm, p, st);
+    if (c.mode == 2) return launch<256, 1, 2, EPI>(tm, p, sm_count, st);
+    return c.cg == 2 ? launch<256, 2, 0, EPI>(tm, p, sm_count, st) : launch<256, 1, 0, EPI>(tm, p, sm_count, st);
 }
 
 // How many clusters of `cluster` CTAs with `warps` warps of the norm kernel run at once: asked once per device, type and shape.
@@ -684,6 +757,43 @@ static int launch_config(const Config& c, const TensorMaps& tm, const GemmParams
     if (c.mode == 4) return launch<256, 1, 4>(tm, p, sm_count, st);
     if (c.cg == 2) return launch<256, 2, 0>(tm, p, sm_count, st);
     return c.tile_n == 256 ? launch<256, 1, 0>(tm, p, sm_count, st) : launch<128, 1, 0>(tm, p, sm_count, st);
+}
+
+// The kernel's parameters for a call without partial sums in a workspace, to one destination.
+static GemmParams gemm_params(const Config& cfg, int tile_cols, const float* a_scale, const float* b_scale, void* C, int M, int N, int K, int n0,
+                              int n_total, unsigned int* status, cudaStream_t stream)
+{
+    GemmParams p{};
+    p.a_scale = a_scale;
+    p.b_scale = b_scale;
+    p.C = static_cast<__nv_bfloat16*>(C);
+    p.partials = nullptr;
+    p.counters = nullptr;
+    p.status = status;
+    p.M = M; p.N = N; p.K = K;
+    p.rows = M;
+    p.n_off = n0;
+    p.sn = ceil_div(n_total, 128);
+    p.m_tiles = ceil_div(M, 128 * cfg.cg);
+    p.n_tiles = ceil_div(N, tile_cols);
+    p.group = tile_group(p.m_tiles, cfg.cg, static_cast<long long>(M) * K);
+    p.group_tiles = p.group * p.n_tiles;
+    p.inv_group_tiles = 1.0f / static_cast<float>(p.group_tiles);
+    p.inv_group = 1.0f / static_cast<float>(p.group);
+    p.inv_last_group = (p.m_tiles % p.group) ? 1.0f / static_cast<float>(p.m_tiles % p.group) : p.inv_group;
+    p.splits = cfg.splits;
+    p.n_dest = 1;
+    p.elem_scale = 1.0f;
+#ifdef FP8BS_PROFILE
+    static long long* prof_buf = nullptr;           // profiling builds only: 8 counters per CTA, read by fp8bs_debug_prof
+    if (!prof_buf) cudaMalloc(&prof_buf, 16 * 1024 * sizeof(long long));
+    cudaMemsetAsync(prof_buf, 0, 16 * 1024 * sizeof(long long), stream);
+    p.prof = prof_buf;
+    g_prof_buf = prof_buf;
+#else
+    (void)stream;
+#endif
+    return p;
 }
 
 // `dests` / `n_dest`: null / 0 for the ordinary call (C is an M x N buffer of its own); otherwise n_dest buffers of
@@ -760,40 +870,65 @@ static int gemm_impl(const void* A, const void* B, const float* a_scale, const f
             if ((rc = encode_c_map(&tm.C.m[d], static_cast<__nv_bfloat16*>(dests[d]) + n0, M, N, n_total))) return rc;
     } else if (cfg.mode != 5 && (rc = encode_c_map(&tm.C.m[0], C, M, N, N))) return rc;
 
-    GemmParams p;
-    p.a_scale = a_scale;
-    p.b_scale = b_scale;
-    p.C = static_cast<__nv_bfloat16*>(C);
-    p.partials = nullptr;
-    p.counters = nullptr;
-    p.status = dev->status_ptr;
-    p.M = M; p.N = N; p.K = K;
-    p.n_off = n0;
-    p.sn = ceil_div(n_total, 128);
-    p.m_tiles = ceil_div(M, 128 * cfg.cg);
-    p.n_tiles = ceil_div(N, cfg.tile_n);
-    p.group = tile_group(p.m_tiles, cfg.cg, static_cast<long long>(M) * K);
-    p.group_tiles = p.group * p.n_tiles;
-    p.inv_group_tiles = 1.0f / static_cast<float>(p.group_tiles);
-    p.inv_group = 1.0f / static_cast<float>(p.group);
-    p.inv_last_group = (p.m_tiles % p.group) ? 1.0f / static_cast<float>(p.m_tiles % p.group) : p.inv_group;
-    p.splits = cfg.splits;
-    p.n_dest = dests ? n_dest : 1;
-    p.elem_scale = 1.0f;
-#ifdef FP8BS_PROFILE
-    {
-        static long long* prof_buf = nullptr;       // profiling builds only: 8 counters per CTA, read by fp8bs_debug_prof
-        if (!prof_buf) cudaMalloc(&prof_buf, 16 * 1024 * sizeof(long long));
-        cudaMemsetAsync(prof_buf, 0, 16 * 1024 * sizeof(long long), static_cast<cudaStream_t>(stream));
-        p.prof = prof_buf;
-        g_prof_buf = prof_buf;
-    }
-#endif
+    GemmParams p = gemm_params(cfg, cfg.tile_n, a_scale, b_scale, C, M, N, K, n0, n_total, dev->status_ptr, st);
+    if (dests) p.n_dest = n_dest;
     if (cfg.mode == 1 || cfg.mode == 3) {
         p.counters = static_cast<unsigned int*>(workspace);
         p.partials = reinterpret_cast<float4*>(static_cast<char*>(workspace) + COUNTER_BYTES);
     }
     return launch_config(cfg, tm, p, dev->sm_count, st);
+}
+
+// The fused calls.  B2 NULL: one product with bias, activation and residual; else the gated pair, in 8 bits where out_scale is given.
+static int fused_impl(const void* A, const void* B, const void* B2, const float* a_scale, const float* b_scale, const float* b2_scale, void* out,
+                      float* out_scale, int M, int N, int K, int rows, const void* bias, int bias_is_bf16, int activation, const void* residual,
+                      long long ldr, float fp8_max, int splits, int tile_n, void* stream)
+{
+    const bool gated = B2 != nullptr, fp8 = out_scale != nullptr;
+    if (!A || !B || !a_scale || !b_scale || !out) return FP8BS_ERR_NULL;
+    int rc = check_shape(M, N, K);
+    if (rc) return rc;
+    if (rows <= 0 || rows > M || (fp8 && N % 128 != 0)) return FP8BS_ERR_SHAPE;
+    if (activation < FP8BS_ACT_NONE || activation > FP8BS_ACT_GELU_TANH) return FP8BS_ERR_ARG;
+    if (fp8 && (!(fp8_max > 0.0f) || fp8_max > 448.0f)) return FP8BS_ERR_ARG;
+    if (residual && ldr < N) return FP8BS_ERR_ARG;
+    auto off = [](const void* q, unsigned bytes) { return (reinterpret_cast<uintptr_t>(q) & (bytes - 1)) != 0; };
+    if (off(A, 16) || off(B, 16) || off(B2, 16) || off(out, 16) || off(a_scale, 16) || off(b_scale, 4) || off(b2_scale, 4) || off(out_scale, 4) ||
+        off(bias, 16) || off(residual, 16) || (residual && ldr % 8 != 0))
+        return FP8BS_ERR_ALIGN;
+    DeviceInfo* dev = nullptr;
+    const int dev_rc = device_setup(&dev);
+    Config cfg{};
+    if ((rc = choose_fused(dev_rc == FP8BS_OK ? dev->model : kB200Model, M, N, K, gated, splits, tile_n, &cfg))) return rc;
+    if (dev_rc) return dev_rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    TensorMaps tm{};
+    if ((rc = cfg.mode == 5 ? encode_few_rows_map(&tm.A, A, M, K, M <= 32 ? 32 : 64) : encode_operand_map(&tm.A, A, M, K))) return rc;
+    if ((rc = encode_operand_map(&tm.B, B, N, K))) return rc;
+    if (gated && (rc = encode_operand_map(&tm.C.m[MAP_UP], B2, N, K))) return rc;
+    if (cfg.mode != 5 && (rc = fp8 ? encode_operand_map(&tm.C.m[0], out, M, N) : encode_c_map(&tm.C.m[0], out, rows, N, N))) return rc;
+    if (residual && cfg.mode == 0 && (rc = encode_c_map(&tm.C.m[MAP_RESIDUAL], const_cast<void*>(residual), rows, N, ldr))) return rc;
+    GemmParams p = gemm_params(cfg, gated ? 128 : cfg.tile_n, a_scale, b_scale, out, M, N, K, 0, N, dev->status_ptr, st);
+    p.rows = rows;
+    Epilogue& e = p.epi;
+    e.bias = bias;
+    e.residual = static_cast<const __nv_bfloat16*>(residual);
+    e.ldr = ldr;
+    e.up_scale = b2_scale;
+    e.q_out = static_cast<uint8_t*>(out);
+    e.scale_out = out_scale;
+    e.bias_is_bf16 = bias_is_bf16;
+    e.fp8_max = fp8_max;
+    const double log2e = 1.4426950408889634, c = 2.0 * 0.7978845608028654;             // 2 sqrt(2 / pi)
+    switch (activation) {
+        case FP8BS_ACT_RELU: e.act = ACT_RELU; break;
+        case FP8BS_ACT_SILU: e.act = ACT_LOGISTIC; e.a = static_cast<float>(-log2e); e.b = 0.0f; break;
+        case FP8BS_ACT_GELU: e.act = ACT_ERF; break;
+        case FP8BS_ACT_GELU_TANH: e.act = ACT_LOGISTIC; e.a = static_cast<float>(-log2e * c); e.b = static_cast<float>(-log2e * c * 0.044715); break;
+        default: e.act = ACT_NONE;
+    }
+    if (!gated) return launch_bias_act(cfg, tm, p, dev->sm_count, st);
+    return fp8 ? launch_gated<EPI_GATED_FP8>(cfg, tm, p, dev->sm_count, st) : launch_gated<EPI_GATED>(cfg, tm, p, dev->sm_count, st);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -988,6 +1123,23 @@ int fp8bs_gemm_ref(const void* A, const void* B, const float* a_scale, const flo
     g_launches.fetch_add(1, std::memory_order_relaxed);
     CUDA_TRY(cudaGetLastError());
     return FP8BS_OK;
+}
+
+int fp8bs_gemm_bias_act(const void* A, const void* B, const float* a_scale, const float* b_scale, void* C, int M, int N, int K, int rows,
+                        const void* bias, int bias_is_bf16, int activation, const void* residual, long long ld_residual, int splits,
+                        int tile_n, void* stream)
+{
+    return fused_impl(A, B, nullptr, a_scale, b_scale, nullptr, C, nullptr, M, N, K, rows, bias, bias_is_bf16, activation, residual, ld_residual,
+                      448.0f, splits, tile_n, stream);
+}
+
+int fp8bs_gemm_gated(const void* A, const void* B_gate, const void* B_up, const float* a_scale, const float* gate_scale, const float* up_scale,
+                     void* H, float* h_scale, int M, int N, int K, int rows, int activation, float fp8_max, int splits, int tile_n,
+                     void* stream)
+{
+    if (!B_up || !up_scale) return FP8BS_ERR_NULL;
+    return fused_impl(A, B_gate, B_up, a_scale, gate_scale, up_scale, H, h_scale, M, N, K, rows, nullptr, 0, activation, nullptr, 0, fp8_max,
+                      splits, tile_n, stream);
 }
 
 int fp8bs_select_path(int M, int N, int K, int* splits, int* tile_n)

@@ -3,7 +3,7 @@
 // A is M x K column-major fp8 e4m3, B is N x K column-major fp8 e4m3, C is bf16 row-major
 // (the operand layouts of the reference kernels, mn_large.hip:11-15 and mn_small.hip:10-17).
 //
-// One kernel template, three parameters:
+// One kernel template, four parameters:
 //   BN      width of the output tile (128 or 256 columns)
 //   CG      1: a CTA owns a 128 x BN tile.  2: two CTAs of a cluster own a 256 x BN tile; each
 //           loads its own 128 rows of A and its own half of the B columns, the leader issues
@@ -27,6 +27,9 @@
 //                 buffers and are handed over once per tile; a promotion thread reads both K blocks of 64 of its
 //                 columns with two loads in flight, scales and adds them in registers and stages the result, then the
 //                 other 64.  One barrier round trip per tile instead of one per K block, and no running sums.
+//   EPI     0: C is the sum.  EPI_BIAS_ACT (modes 0 and 2): C = act(sum + bias) + residual in fp32, rounded once.  EPI_GATED,
+//           EPI_GATED_FP8 (modes 0 and 2, 256-wide tiles): the tile is 128 columns of two products with the same A, h = act(first) *
+//           second is stored, in bf16 or in 8 bits with 1 x 128 scales in the layout of A.  See "fused epilogues" below.
 // The epilogue stores a finished tile to one or several destinations (CMaps): the caller's C, and
 // for the fused distribution of an N-sharded GEMM the peer-mapped C of the other GPUs.
 //
@@ -68,6 +71,7 @@
 // is released.
 #pragma once
 #include "ptx.cuh"
+#include "epilogue.cuh"
 #include <cuda_bf16.h>
 #include <cstdint>
 
@@ -106,11 +110,26 @@ struct GemmParams {
     float inv_group_tiles;   // their reciprocals, and that of the last (shorter) group's height
     float inv_group, inv_last_group;
     int n_dest;              // number of valid entries of the CMaps argument (1 = only the caller's C)
+    int rows;                // rows of C that exist: M, fewer in the fused calls
     float elem_scale;        // folded into b_scale: 1 for e4m3fn bytes
+    Epilogue epi;            // EPI != 0 only
 #ifdef FP8BS_PROFILE
     long long* prof;         // per CTA: 8 cycle counters (profiling builds only)
 #endif
 };
+
+// Fused epilogues.  What they need besides C is brought in under the K loop of the tile: the residual by TMA into the warp's
+// staging boxes, where the result replaces it, the bias by cp.async into 512 bytes per warp.
+// Gated: the two matrices are the two halves of the tile's B operand.  With a pair the leader loads 128 columns of the first and the
+// peer the same columns of the second; part h of the tile (64 columns from each CTA's slab, see col_of) is then 64 columns of the
+// first product beside the same 64 of the second, and a promotion thread owns both.  A single CTA loads both slabs, hands the tile
+// over as one part, and its column group g takes columns 64 g .. of each slab.  A tile is exactly one scale block of h wide: its
+// two column groups exchange their rows' largest magnitudes through shared memory.
+enum : int { EPI_NONE = 0, EPI_BIAS_ACT = 1, EPI_GATED = 2, EPI_GATED_FP8 = 3 };
+constexpr int EPI_BIAS_BYTES = 8 * 512;              // per promotion warp: the bias of its columns (gated fp8: [column group][row] magnitudes)
+constexpr int epi_smem(int epi) { return epi == EPI_NONE ? 0 : EPI_BIAS_BYTES; }
+// CMaps entries of the fused calls behind C (entry 0; gated fp8: the bytes of h)
+constexpr int MAP_RESIDUAL = 1, MAP_UP = 1;
 
 template <int BN, int CG>
 struct TileCfg {
@@ -145,7 +164,8 @@ struct TileCfg {
     static constexpr int STAGES = (SMEM_LIMIT - FIXED) / STAGE_BYTES;
     static_assert(STAGES >= 2, "pipeline depth");
     static constexpr int NUM_BARS = 2 * STAGES + 2 * NBUF * NH;
-    static_assert(NUM_BARS * 8 + 64 <= 512, "barrier area");
+    static_assert((NUM_BARS + PROMO_WARPS) * 8 + 16 <= 512, "barrier area");    // EPI_BIAS_ACT: one more per promotion warp
+    static_assert(FIXED + STAGES * STAGE_BYTES + EPI_BIAS_BYTES <= SMEM_LIMIT, "room for the fused epilogues");
     static constexpr int SMEM_BYTES = FIXED + STAGES * STAGE_BYTES;
 };
 
@@ -299,6 +319,60 @@ __device__ __forceinline__ void stage_and_store_2x64(const CUtensorMap* tmC, int
     }
 }
 
+// 64 columns of this thread's row, two fp32 per register pair.
+typedef unsigned long long Cols64[2][16];
+
+template <class F>
+__device__ __forceinline__ unsigned long long each_f32(unsigned long long v, F f)
+{
+    return pack_f32x2(f(f32x2_lo(v)), f(f32x2_hi(v)));
+}
+// v = act(v + bias): bias from shared memory (64 fp32), or none.
+template <int ACT>
+__device__ __forceinline__ void bias_and_activate(unsigned long long (&v)[16], uint32_t bias_addr, bool has_bias, const Epilogue& e)
+{
+    if (has_bias)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            unsigned long long b0, b1;
+            ptx::ld_shared_v2_b64(bias_addr + static_cast<uint32_t>(16 * i), b0, b1);
+            v[2 * i] = pack_f32x2(f32x2_lo(v[2 * i]) + f32x2_lo(b0), f32x2_hi(v[2 * i]) + f32x2_hi(b0));
+            v[2 * i + 1] = pack_f32x2(f32x2_lo(v[2 * i + 1]) + f32x2_lo(b1), f32x2_hi(v[2 * i + 1]) + f32x2_hi(b1));
+        }
+    if constexpr (ACT != ACT_NONE)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = each_f32(v[i], [&](float x) { return activate<ACT>(x, e); });
+}
+// stage_64 onto the residual that lies in the box.
+__device__ __forceinline__ void add_and_stage_64(uint8_t* stg, int lane, const unsigned long long (&c0)[16], const unsigned long long (&c1)[16])
+{
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        uint4* at = reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4));
+        const uint4 r = *at;
+        auto add = [&](int i, uint32_t w) {
+            const unsigned long long v = (i < 16) ? c0[i & 15] : c1[i & 15];
+            return pack_bf16x2(f32x2_lo(v) + __uint_as_float(w << 16), f32x2_hi(v) + __uint_as_float(w & 0xffff0000u));
+        };
+        *at = make_uint4(add(4 * j, r.x), add(4 * j + 1, r.y), add(4 * j + 2, r.z), add(4 * j + 3, r.w));
+    }
+}
+// A barrier of the promotion warps; whether `fail` holds for any of them.  Every promotion warp has to come here, aborting or not.
+template <int THREADS>
+__device__ __forceinline__ bool promo_any(bool fail)
+{
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred.aligned q, 1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(fail ? 1u : 0u), "n"(THREADS)
+        : "memory");
+    return r != 0u;
+}
+
 // Self-test of the failure path: one warp waits, with a short limit, on a barrier that nothing ever arrives on.
 // The wait must give up, record DS_TIMEOUT_SELFTEST in the status word and the kernel must end normally.
 constexpr uint32_t DS_TIMEOUT_SELFTEST = 9;
@@ -317,7 +391,7 @@ __global__ void wait_timeout_selftest_kernel(unsigned int* status, long long lim
     (void)ok;
 }
 
-template <int BN, int CG, int MODE>
+template <int BN, int CG, int MODE, int EPI = EPI_NONE>
 __global__ void __launch_bounds__(TileCfg<BN, CG>::THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
             const __grid_constant__ CMaps cmaps, const GemmParams p)
@@ -325,7 +399,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     using Cfg = TileCfg<BN, CG>;
     constexpr int STAGES = Cfg::STAGES;
     constexpr int NBUF = Cfg::NBUF;
-    constexpr int NH = Cfg::NH;
+    constexpr bool GATED = (EPI == EPI_GATED || EPI == EPI_GATED_FP8);
+    static_assert(EPI == EPI_NONE || MODE == 0 || MODE == 2, "fused epilogues: the full-K kernel and the cluster reduction");
+    static_assert(!GATED || BN == 256, "gated: two slabs of 128 columns");
+    constexpr bool WHOLE = GATED && CG == 1;            // both slabs are handed over together
+    constexpr int NH = WHOLE ? 1 : Cfg::NH;
+    constexpr int TILE_N = GATED ? 128 : BN;            // columns of C a tile covers
     constexpr bool SPLITK = (MODE == 1 || MODE == 2);   // K cut into p.splits equal ranges per tile
     constexpr bool STREAMK = (MODE == 3);               // K blocks of all tiles dealt out evenly, see below
     static_assert(MODE != 2 || CG == 1, "the cluster reduction uses the cluster for the K splits");
@@ -353,6 +432,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
     auto tfull_bar = [&](int h, int b) { return bar_base + 8u * (2 * STAGES + h * NBUF + b); };
     auto tempty_bar = [&](int h, int b) { return bar_base + 8u * (2 * STAGES + (NH + h) * NBUF + b); };
+    auto residual_bar = [&](int w) { return bar_base + 8u * (Cfg::NUM_BARS + w) + 16u; };     // EPI_BIAS_ACT, behind the control words
+    const uint32_t epi_base = bar_base + 512u;
 
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);   // uniform, and known to be
     const int lane = threadIdx.x & 31;
@@ -366,6 +447,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         ptx::prefetch_tensormap(&tmA);
         ptx::prefetch_tensormap(&tmB);
         for (int d = 0; d < p.n_dest; ++d) ptx::prefetch_tensormap(&cmaps.m[d]);
+        if (GATED || (EPI == EPI_BIAS_ACT && MODE == 0 && p.epi.residual)) ptx::prefetch_tensormap(&cmaps.m[1]);
         for (int s = 0; s < STAGES; ++s) {
             ptx::mbar_init(full_bar(s), 1);
             ptx::mbar_init(empty_bar(s), 1);
@@ -375,6 +457,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 ptx::mbar_init(tfull_bar(h, b), 2);                                // the MMA warp's commit and the scale warp
                 ptx::mbar_init(tempty_bar(h, b), Cfg::PROMO_WARPS / NH * CG);      // the leader also hears from the peer's warps
             }
+        if constexpr (EPI != EPI_NONE)
+            for (int w = 0; w < Cfg::PROMO_WARPS; ++w) ptx::mbar_init(residual_bar(w), 1);
         ctrl[1] = 0u;
         ctrl[2] = 0u;
         ptx::fence_mbar_init();
@@ -450,7 +534,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         divide(rem, left < p.group ? left : p.group, left < p.group ? p.inv_last_group : p.inv_group, ni, mi);
         mi += first;
         m0 = mi * Cfg::TILE_M + static_cast<int>(rank) * Cfg::BM;
-        n0 = ni * BN;
+        n0 = ni * TILE_N;
     };
 
     // First column, within the tile, of the 64-column piece q of column group g.  A pair's MMA of part h takes 64 columns
@@ -468,10 +552,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             for (int u = unit0; u < units && ok; u += unit_step) {
                 int tile, m0, n0, kb0, kb1;
                 decode(u, tile, m0, n0, kb0, kb1);
-                const int nb0 = n0 + static_cast<int>(rank) * Cfg::B_COLS;    // first B column this CTA loads
+                const int nb0 = GATED ? n0 : n0 + static_cast<int>(rank) * Cfg::B_COLS;    // first B column this CTA loads
                 int nbox = (p.N - nb0 + 127) >> 7;                            // B slabs that hold any real column
                 nbox = nbox < 0 ? 0 : (nbox < Cfg::NBOX_B ? nbox : Cfg::NBOX_B);
-                if (CG == 2) nbox = Cfg::NBOX_B;                              // pairs: fixed byte count (zero fill)
+                if (CG == 2 || GATED) nbox = Cfg::NBOX_B;                     // pairs: fixed byte count (zero fill)
                 for (int kb = kb0; kb < kb1; ++kb, ++it) {
                     const int s = stage;
                     const uint32_t ph = sphase;
@@ -487,13 +571,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                         const uint32_t lead_full = ptx::mapa(full_bar(s), 0);
                         if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(s), 2 * Cfg::STAGE_BYTES);
                         ptx::tma_load_2d_pair(a_dst, &tmA, m0, kb * Cfg::BK, lead_full);
+                        const CUtensorMap* tmb = GATED && rank ? &cmaps.m[MAP_UP] : &tmB;
                         for (int j = 0; j < Cfg::NBOX_B; ++j)
-                            ptx::tma_load_2d_pair(a_dst + Cfg::SLAB * (1 + j), &tmB, nb0 + 128 * j, kb * Cfg::BK, lead_full);
+                            ptx::tma_load_2d_pair(a_dst + Cfg::SLAB * (1 + j), tmb, nb0 + 128 * j, kb * Cfg::BK, lead_full);
                     } else {
                         ptx::mbar_arrive_expect_tx(full_bar(s), Cfg::SLAB * (1 + nbox));
                         ptx::tma_load_2d(a_dst, &tmA, m0, kb * Cfg::BK, full_bar(s));
                         for (int j = 0; j < nbox; ++j)
-                            ptx::tma_load_2d(a_dst + Cfg::SLAB * (1 + j), &tmB, nb0 + 128 * j, kb * Cfg::BK, full_bar(s));
+                            ptx::tma_load_2d(a_dst + Cfg::SLAB * (1 + j), GATED && j ? &cmaps.m[MAP_UP] : &tmB, GATED ? nb0 : nb0 + 128 * j,
+                                             kb * Cfg::BK, full_bar(s));
                     }
                 }
             }
@@ -623,7 +709,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     int tile, m0, n0;
                     decode(fu, tile, m0, n0, fkb, fkb1);
                     fm = m0 + lane;
-                    fnb = (p.n_off + n0 + (lane & (NQ - 1)) * 64) >> 7;
+                    fnb = GATED ? n0 >> 7 : (p.n_off + n0 + (lane & (NQ - 1)) * 64) >> 7;
                     fnb = fnb < p.sn ? fnb : p.sn - 1;
                 }
             };
@@ -633,7 +719,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 const float* ap = p.a_scale + static_cast<size_t>(fkb) * p.M + fm;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) a[j] = (fm + 32 * j < p.M) ? __ldg(ap + 32 * j) : 0.0f;
-                b = __ldg(p.b_scale + static_cast<size_t>(fkb) * p.sn + fnb);
+                b = __ldg((GATED && (lane & 1) ? p.epi.up_scale : p.b_scale) + static_cast<size_t>(fkb) * p.sn + fnb);
                 if (++fkb == fkb1) {
                     fu += unit_step;
                     fetch_unit();
@@ -667,7 +753,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
                             float* w = dst + (g * 128 + 32 * j) * Cfg::QUADS;
-                            if constexpr (Cfg::QUADS == 2)
+                            if constexpr (GATED)            // lanes 0 and 1: the scale of the first and of the second matrix
+                                *reinterpret_cast<float2*>(w) = make_float2(av[d][j] * bs[0], av[d][j] * bs[1]);
+                            else if constexpr (Cfg::QUADS == 2)
                                 *reinterpret_cast<float2*>(w) = make_float2(av[d][j] * bs[col_of(g, 0) / 64], av[d][j] * bs[col_of(g, 1) / 64]);
                             else *w = av[d][j] * bs[g];
                         }
@@ -704,8 +792,20 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         for (int u = unit0; u < units; u += unit_step) {
             int tile, m0, n0, kb0, kb1;
             decode(u, tile, m0, n0, kb0, kb1);
-            const int ncol0 = n0 + col_of(grp, 0);            // first local columns of this thread's pieces
+            const int ncol0 = GATED ? n0 + grp * 64 : n0 + col_of(grp, 0);      // first local columns of this thread's pieces
             const int ncol1 = n0 + col_of(grp, 1);
+            if constexpr (EPI == EPI_BIAS_ACT && MODE == 0)
+                if (p.epi.bias) {
+                    // the bias of this warp's columns, four per lane; the last tile's has been used (its staging ended in a __syncwarp)
+                    const int c = (lane < 16 ? ncol0 : ncol1) + (lane & 15) * 4;
+                    const bool valid = c < p.N && lane < 16 * Cfg::QUADS;
+                    const uint32_t dst = epi_base + static_cast<uint32_t>(pw * 512);
+                    if (p.epi.bias_is_bf16)
+                        ptx::cp_async_8(dst + lane * 8, static_cast<const __nv_bfloat16*>(p.epi.bias) + (valid ? c : 0), valid);
+                    else
+                        ptx::cp_async_16(dst + lane * 16, static_cast<const float*>(p.epi.bias) + (valid ? c : 0), valid);
+                }
+            const bool residual_here = EPI == EPI_BIAS_ACT && p.epi.residual && ncol0 < p.N && m0 + quarter * 32 < p.rows;
             // running sums of this thread's row: 4 chunks of 32 columns, two fp32 per 64-bit register
             unsigned long long acc[Cfg::NCH][16];
 #pragma unroll
@@ -755,7 +855,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     if (last_unit) {
                         // the CTA's last tile: each store leaves as soon as its box is staged (shorter tail)
                         stage_and_store_64<-1>(cmaps.m, p.n_dest, my_stg + h * 4096, my_stg_addr + h * 4096, lane,
-                                               PackedCols{acc[0], acc[1]}, ncol0 + h * 64, m0 + quarter * 32, p.M, p.N);
+                                               PackedCols{acc[0], acc[1]}, ncol0 + h * 64, m0 + quarter * 32, p.rows, p.N);
                     } else {
                         stage_64(my_stg + h * 4096, lane, PackedCols{acc[0], acc[1]});
                     }
@@ -763,7 +863,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 if (!last_unit) {
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
-                    if (ncol0 < p.N && m0 + quarter * 32 < p.M && ptx::elect_one()) {
+                    if (ncol0 < p.N && m0 + quarter * 32 < p.rows && ptx::elect_one()) {
                         for (int d = 0; d < p.n_dest; ++d) {
                             ptx::tma_store_2d(cmaps.m + d, my_stg_addr, ncol0, m0 + quarter * 32);
                             if (ncol0 + 64 < p.N) ptx::tma_store_2d(cmaps.m + d, my_stg_addr + 4096, ncol0 + 64, m0 + quarter * 32);
@@ -787,7 +887,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 PROF_T0();
                 ptx::tc_fence_after_sync();
                 const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                       static_cast<uint32_t>(b * BN + grp * Cfg::COLS);
+                                       static_cast<uint32_t>(b * BN + grp * (WHOLE ? 64 : Cfg::COLS));
                 // scale products of this row, one per 64 columns; in flight together with the first TMEM load
                 float sc[Cfg::QUADS];
                 {
@@ -801,7 +901,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 uint32_t v[64];
 #pragma unroll
                 for (int q = 0; q < Cfg::COLS / 64; ++q) {
-                    ptx::tmem_ld_x64_sync(taddr + q * 64, v);
+                    ptx::tmem_ld_x64_sync(taddr + q * (WHOLE ? 128 : 64), v);
                     if (q == Cfg::COLS / 64 - 1) {
                         // The last columns of the buffer are in registers: hand the TMEM buffer back now, so that
                         // the hand-off to the MMA warp overlaps the FMAs below instead of following them.
@@ -815,6 +915,16 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     const unsigned long long s2 = pack_f32x2(sc[q], sc[q]);
                     ptx::fma32_from64<0>(acc[2 * q], v, s2);
                     ptx::fma32_from64<32>(acc[2 * q + 1], v, s2);
+                }
+                if constexpr (EPI == EPI_BIAS_ACT && MODE == 0) {
+                    // the residual comes into the boxes the result leaves from, once the stores of the tile before have read them
+                    if (kb == kb0 && residual_here && ptx::elect_one()) {
+                        ptx::tma_store_wait_read<0>();
+                        ptx::mbar_arrive_expect_tx(residual_bar(pw), 4096u * ((Cfg::NSTG == 2 && ncol1 < p.N) ? 2 : 1));
+                        ptx::tma_load_2d(my_stg_addr, &cmaps.m[MAP_RESIDUAL], ncol0, m0 + quarter * 32, residual_bar(pw));
+                        if (Cfg::NSTG == 2 && ncol1 < p.N)
+                            ptx::tma_load_2d(my_stg_addr + 4096, &cmaps.m[MAP_RESIDUAL], ncol1, m0 + quarter * 32, residual_bar(pw));
+                    }
                 }
                 if (pw == 0 && lane == 0) PROF_TRACE(5, ait);
                 if (pw == 1 && lane == 0) PROF_TRACE(8, ait);
@@ -834,20 +944,119 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     __syncwarp();
                     if (u + unit_step < units) {
                         stage_and_store_2x64(cmaps.m, p.n_dest, my_stg, my_stg_addr, lane, PackedCols{acc[0], acc[1]},
-                                             PackedCols{acc[2], acc[3]}, ncol0, ncol1, m0 + quarter * 32, p.M, p.N);
+                                             PackedCols{acc[2], acc[3]}, ncol0, ncol1, m0 + quarter * 32, p.rows, p.N);
                     } else {
                         // the CTA's last tile: the first store leaves while the second box is being staged (shorter tail)
                         stage_and_store_64<-1>(cmaps.m, p.n_dest, my_stg, my_stg_addr, lane, PackedCols{acc[0], acc[1]},
-                                               ncol0, m0 + quarter * 32, p.M, p.N);
+                                               ncol0, m0 + quarter * 32, p.rows, p.N);
                         stage_and_store_64<-1>(cmaps.m, p.n_dest, my_stg + 4096, my_stg_addr + 4096, lane,
-                                               PackedCols{acc[2], acc[3]}, ncol1, m0 + quarter * 32, p.M, p.N);
+                                               PackedCols{acc[2], acc[3]}, ncol1, m0 + quarter * 32, p.rows, p.N);
                     }
                 } else {
                     stage_and_store_64<0>(cmaps.m, p.n_dest, my_stg, my_stg_addr, lane, PackedCols{acc[0], acc[1]}, ncol0,
-                                          m0 + quarter * 32, p.M, p.N);
+                                          m0 + quarter * 32, p.rows, p.N);
                 }
             };
-            if constexpr (MODE == 0) {
+            if constexpr (MODE == 0 && EPI == EPI_BIAS_ACT) {
+                if (!ok) break;
+                const uint32_t bias = epi_base + static_cast<uint32_t>(pw * 512);
+                if (p.epi.bias) {
+                    ptx::cp_async_wait_all();
+                    if (p.epi.bias_is_bf16) {
+                        // widened in place: a lane's own four, after every lane has read its own
+                        uint2* raw = reinterpret_cast<uint2*>(stg_ptr + (bias - stg_base));
+                        const uint2 w = raw[lane];
+                        __syncwarp();
+                        reinterpret_cast<uint4*>(raw)[lane] = make_uint4(w.x << 16, w.x & 0xffff0000u, w.y << 16, w.y & 0xffff0000u);
+                    }
+                    __syncwarp();
+                }
+                with_activation(p.epi, [&](auto act) {
+#pragma unroll
+                    for (int c = 0; c < Cfg::NCH; ++c)
+                        bias_and_activate<decltype(act)::value>(acc[c], bias + c * 128, p.epi.bias != nullptr, p.epi);
+                });
+                if (residual_here) {
+                    ok = wait_bounded(residual_bar(pw), tcount & 1u, abort_flag, p.status, DS_TIMEOUT_STAGE_FULL);
+                    ok = __all_sync(0xffffffffu, ok);
+                    ++tcount;                                           // residuals waited for
+                    if (!ok) break;
+                    add_and_stage_64(my_stg, lane, acc[0], acc[1]);
+                    if constexpr (Cfg::NSTG == 2) add_and_stage_64(my_stg + 4096, lane, acc[2], acc[3]);
+                } else {
+                    // the previous stores have read the boxes before anything is staged into them
+                    if (ptx::elect_one()) ptx::tma_store_wait_read<0>();
+                    __syncwarp();
+                    stage_64(my_stg, lane, PackedCols{acc[0], acc[1]});
+                    if constexpr (Cfg::NSTG == 2) stage_64(my_stg + 4096, lane, PackedCols{acc[2], acc[3]});
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (ncol0 < p.N && m0 + quarter * 32 < p.rows && ptx::elect_one()) {
+                    ptx::tma_store_2d(cmaps.m, my_stg_addr, ncol0, m0 + quarter * 32);
+                    if (Cfg::NSTG == 2 && ncol1 < p.N) ptx::tma_store_2d(cmaps.m, my_stg_addr + 4096, ncol1, m0 + quarter * 32);
+                    ptx::tma_store_commit();
+                }
+            } else if constexpr (MODE == 0 && GATED) {
+                if (EPI == EPI_GATED && !ok) break;
+                // h = act(first) * second, in the registers of the first
+                with_activation(p.epi, [&](auto act) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const unsigned long long g = acc[c][i], up = acc[c + 2][i];
+                            acc[c][i] = pack_f32x2(activate<decltype(act)::value>(f32x2_lo(g), p.epi) * f32x2_lo(up),
+                                                   activate<decltype(act)::value>(f32x2_hi(g), p.epi) * f32x2_hi(up));
+                        }
+                });
+                // two boxes (or two 16 KB tiles of bytes), used in turn
+                const uint32_t turn = tcount++ & 1u;
+                if constexpr (EPI == EPI_GATED) {
+                    if (ptx::elect_one()) ptx::tma_store_wait_read<1>();
+                    __syncwarp();
+                    stage_64(my_stg + turn * 4096, lane, PackedCols{acc[0], acc[1]});
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (ptx::elect_one()) {
+                        if (ncol0 < p.N && m0 + quarter * 32 < p.rows) ptx::tma_store_2d(cmaps.m, my_stg_addr + turn * 4096, ncol0, m0 + quarter * 32);
+                        ptx::tma_store_commit();                        // an empty group too: groups are counted above
+                    }
+                } else {
+                    float* row_max = reinterpret_cast<float*>(stg_ptr + (epi_base - stg_base)) + row_in_tile;       // [column group][row]
+                    float mine = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            mine = max_nan(mine, max_nan(fabsf(f32x2_lo(acc[c][i])), fabsf(f32x2_hi(acc[c][i]))));
+                    row_max[grp * 128] = mine;
+                    // warp 0 of these issues the stores: the one before the last has read its tile of bytes
+                    if (pw == 0 && ptx::elect_one()) ptx::tma_store_wait_read<1>();
+                    if (promo_any<Cfg::PROMO_THREADS>(!ok)) { ok = false; break; }
+                    float inverse;
+                    const float f = scale_factor(max_nan(mine, row_max[(grp ^ 1) * 128]), p.epi.fp8_max, inverse);
+                    if (grp == 0 && m0 + row_in_tile < p.M && n0 < p.N)
+                        p.epi.scale_out[static_cast<size_t>(n0 >> 7) * p.M + m0 + row_in_tile] = inverse;
+                    // byte (k, row) of the tile, as a 128-byte-swizzled store box {128 rows, 128 k} expects it
+                    uint8_t* bytes = stg_ptr + turn * 16384 + grp * 64 * 128 + (row_in_tile & 15);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const uint32_t q = cvt_e4m3x2(f32x2_lo(acc[c][i]) * f, f32x2_hi(acc[c][i]) * f);
+                            const int k = c * 32 + 2 * i;
+                            bytes[k * 128 + (((row_in_tile >> 4) ^ (k & 7)) << 4)] = static_cast<uint8_t>(q);
+                            bytes[(k + 1) * 128 + (((row_in_tile >> 4) ^ ((k + 1) & 7)) << 4)] = static_cast<uint8_t>(q >> 8);
+                        }
+                    ptx::fence_proxy_async_smem();
+                    asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(Cfg::PROMO_THREADS) : "memory");
+                    if (pw == 0 && ptx::elect_one()) {
+                        if (m0 < p.M) ptx::tma_store_2d(cmaps.m, stg_base + turn * 16384, m0, n0);
+                        ptx::tma_store_commit();                        // an empty group too: groups are counted above
+                    }
+                }
+            } else if constexpr (MODE == 0) {
                 if (!ok) break;
                 store_tile();
             } else if constexpr (MODE == 3) {
@@ -1000,7 +1209,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                                 sum[4 * j + 3] += v.w;
                             }
                         }
-                        stage_and_store_64<0>(cmaps.m, p.n_dest, my_stg, my_stg_addr, lane, FloatCols{sum}, h ? ncol1 : ncol0, m0 + quarter * 32, p.M, p.N);
+                        stage_and_store_64<0>(cmaps.m, p.n_dest, my_stg, my_stg_addr, lane, FloatCols{sum}, h ? ncol1 : ncol0, m0 + quarter * 32, p.rows, p.N);
                     }
                 }
             }
@@ -1013,6 +1222,14 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         t_epi += 0;
         if (pw == 0 && lane == 0) { PROF_OUT(5, w_tfull); PROF_OUT(6, t_fma); PROF_OUT(7, t_epi); PROF_STAMP(13); }
 #endif
+        if constexpr (EPI == EPI_BIAS_ACT && MODE == 0) {
+            ptx::cp_async_wait_all();
+            if (!ok) {
+                // giving up with a residual possibly in flight: a bounded time to land
+                const long long t0 = clock64();
+                while (clock64() - t0 < 2000000LL) __nanosleep(1000);
+            }
+        }
         // C must have been read out of shared memory before the CTA goes away
         if (ptx::elect_one()) ptx::tma_store_wait_read<0>();
         __syncwarp();
@@ -1027,24 +1244,69 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             const int my = static_cast<int>(ptx::cluster_ctarank());     // = this CTA's split index
             int tile, m0, n0, kb0, kb1;
             decode(static_cast<int>(blockIdx.x), tile, m0, n0, kb0, kb1);
-            const int r0 = (128 * my) / S, r1 = (128 * (my + 1)) / S;     // the rows this CTA finishes
+            // the rows this CTA finishes (gated fp8: pairs of rows)
+            const int r0 = EPI == EPI_GATED_FP8 ? 2 * ((64 * my) / S) : (128 * my) / S;
+            const int r1 = EPI == EPI_GATED_FP8 ? 2 * ((64 * (my + 1)) / S) : (128 * (my + 1)) / S;
             uint32_t peer[8];
 #pragma unroll
             for (int s = 0; s < 8; ++s) peer[s] = ptx::mapa(stage_base, static_cast<uint32_t>(s < S ? s : 0));
-            const int items = (r1 - r0) * (BN / 4);
-            for (int idx = static_cast<int>(threadIdx.x) - 128; idx < items; idx += Cfg::PROMO_THREADS) {
-                const int row = r0 + idx / (BN / 4), c4 = idx % (BN / 4);
-                const uint32_t off = static_cast<uint32_t>(row * PART_PITCH + c4 * 16);
+            auto sum_at = [&](int row, int c) {                         // splits in fixed order: bit-deterministic
+                const uint32_t off = static_cast<uint32_t>(row * PART_PITCH + c * 4);
                 float4 v[8];
 #pragma unroll
                 for (int s = 0; s < 8; ++s)
                     if (s < S) v[s] = ptx::ld_shared_cluster_v4(peer[s] + off);
                 float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                for (int s = 0; s < 8; ++s)              // fixed order 0, 1, .., S-1: bit-deterministic
+                for (int s = 0; s < 8; ++s)
                     if (s < S) { sum.x += v[s].x; sum.y += v[s].y; sum.z += v[s].z; sum.w += v[s].w; }
+                return sum;
+            };
+            if constexpr (GATED) {
+                // A warp takes a row (fp8: two neighbouring ones, a 16-bit store per column), a lane four columns.  Partial tiles are laid
+                // out [column group][first | second][64].
+                constexpr int ROWS = EPI == EPI_GATED_FP8 ? 2 : 1;
+                const int c = lane * 4, part = (c >> 6) * 128 + (c & 63);
+                for (int row = r0 + (warp - 4) * ROWS; row < r1; row += Cfg::PROMO_WARPS * ROWS) {
+                    uint32_t q[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 1
+                    for (int i = 0; i < ROWS; ++i) {
+                        const float4 g = sum_at(row + i, part), up = sum_at(row + i, part + 64);
+                        float4 h;
+                        with_activation(p.epi, [&](auto act) {
+                            constexpr int A = decltype(act)::value;
+                            h = make_float4(activate<A>(g.x, p.epi) * up.x, activate<A>(g.y, p.epi) * up.y, activate<A>(g.z, p.epi) * up.z,
+                                            activate<A>(g.w, p.epi) * up.w);
+                        });
+                        const int m = m0 + row + i;
+                        if constexpr (EPI == EPI_GATED_FP8) {
+                            const float amax = warp_absmax_nan(max_nan(max_nan(fabsf(h.x), fabsf(h.y)), max_nan(fabsf(h.z), fabsf(h.w))));
+                            float inverse;
+                            const float f = scale_factor(amax, p.epi.fp8_max, inverse);
+                            if (lane == 0 && m < p.M) p.epi.scale_out[static_cast<size_t>(n0 >> 7) * p.M + m] = inverse;
+                            const uint32_t lo = cvt_e4m3x2(h.x * f, h.y * f), hi = cvt_e4m3x2(h.z * f, h.w * f);
+                            q[0] |= (lo & 0xffu) << (8 * i);
+                            q[1] |= (lo >> 8) << (8 * i);
+                            q[2] |= (hi & 0xffu) << (8 * i);
+                            q[3] |= (hi >> 8) << (8 * i);
+                        } else if (m < p.rows && n0 + c < p.N) {
+                            *reinterpret_cast<uint2*>(p.C + static_cast<size_t>(m) * p.N + n0 + c) = make_uint2(pack_bf16x2(h.x, h.y), pack_bf16x2(h.z, h.w));
+                        }
+                    }
+                    if constexpr (EPI == EPI_GATED_FP8)
+                        if (m0 + row < p.M)                             // M is a multiple of 16: both rows or none
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                *reinterpret_cast<uint16_t*>(p.epi.q_out + static_cast<size_t>(n0 + c + j) * p.M + m0 + row) = static_cast<uint16_t>(q[j]);
+                }
+            }
+            const int items = GATED ? 0 : (r1 - r0) * (BN / 4);
+            for (int idx = static_cast<int>(threadIdx.x) - 128; idx < items; idx += Cfg::PROMO_THREADS) {
+                const int row = r0 + idx / (BN / 4), c4 = idx % (BN / 4);
+                float4 sum = sum_at(row, c4 * 4);
                 const int m = m0 + row, n = n0 + c4 * 4;
-                if (m < p.M && n < p.N) {
+                if (m < p.rows && n < p.N) {
+                    if constexpr (EPI == EPI_BIAS_ACT) sum = finish_4(sum, p.epi, m, n);
                     uint2 q;
                     q.x = pack_bf16x2(sum.x, sum.y);
                     q.y = pack_bf16x2(sum.z, sum.w);

@@ -21,26 +21,32 @@
 
 namespace fp8bs {
 
-template <int T>
+// EPI: the fused epilogues of gemm_kernel.cuh.  Gated: a K block brings 128 columns of both matrices (a stage of 32 KB of weights, one CTA
+// per SM), a promotion thread owns one column of both products, and all partial sums go through shared memory, so that a warp
+// then holds the 128 columns of a row: one scale block.
+template <int T, int EPI = EPI_NONE>
 struct SmallMCfg {
+    static constexpr bool GATED = (EPI == EPI_GATED || EPI == EPI_GATED_FP8);
+    static constexpr int NW = GATED ? 2 : 1;            // matrices
     static_assert(T == 16 || T == 32 || T == 64, "rows of C a tile has room for");
     static constexpr int X_WIDTH = T < 32 ? 32 : T;     // bytes per k of the box of A, and its swizzle span
     static constexpr int W_BYTES = 128 * 128;           // box of B: 128 columns of C x 128 k
     static constexpr int X_BYTES = 128 * X_WIDTH;
-    static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
-    static constexpr int STAGES = T == 64 ? 3 : 4;
-    static constexpr int NBUF = 4;                      // TMEM buffers of T columns
-    static constexpr int TMEM_COLS = NBUF * T;
+    static constexpr int STAGE_BYTES = NW * W_BYTES + X_BYTES;
+    static constexpr int STAGES = GATED ? (T == 64 ? 3 : 5) : T == 64 ? 3 : 4;
+    static constexpr int NBUF = 4;                      // TMEM buffers of T columns per matrix
+    static constexpr int TMEM_COLS = NBUF * NW * T;
     static constexpr int SSLOTS = 2 * NBUF;             // scale products: [column half][row of C]
     static constexpr int SSLOT_FLOATS = 2 * T;
     static constexpr int SLOT_BYTES = SSLOTS * SSLOT_FLOATS * 4;
-    static constexpr int RED_BYTES = (T + 7) * 512;     // partial sums received: [split][row of C][128 columns]
+    static constexpr int RED_BYTES = (T + 7) * 512 * NW;   // partial sums received: [split][row of C][matrix][128 columns]
     static constexpr int TW = T == 64 ? 32 : 16;        // rows of C of a promotion thread: with one warp per scheduler the
                                                         // instruction count per thread is what the last microsecond is spent on
     static constexpr int PROMO_WARPS = 4 * (T / TW);
     static constexpr int THREADS = 32 * (PROMO_WARPS + 3);
     static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + RED_BYTES + SLOT_BYTES + 256;
-    static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
+    static constexpr int CTAS = GATED ? 1 : 2;          // per SM
+    static_assert(CTAS * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
     static_assert((2 * STAGES + 2 * NBUF) * 8 + 16 <= 256, "barrier area");
 };
 
@@ -70,11 +76,15 @@ __device__ __forceinline__ void tmem_ld_x32_sync(uint32_t taddr, uint32_t (&v)[3
 }
 
 // grid = n_tiles * splits CTAs, cluster size = splits.
-template <int T>
-__global__ void __launch_bounds__(SmallMCfg<T>::THREADS, 2)
-gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const GemmParams p)
+// tmU: the second matrix (gated; otherwise not used).
+template <int T, int EPI = EPI_NONE>
+__global__ void __launch_bounds__((SmallMCfg<T, EPI>::THREADS), (SmallMCfg<T, EPI>::CTAS))
+gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmU,
+                    const GemmParams p)
 {
-    using Cfg = SmallMCfg<T>;
+    using Cfg = SmallMCfg<T, EPI>;
+    constexpr bool GATED = Cfg::GATED;
+    constexpr int NW = Cfg::NW;
     constexpr int STAGES = Cfg::STAGES, NBUF = Cfg::NBUF;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw);
@@ -105,6 +115,7 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     if (threadIdx.x == 0) {
         ptx::prefetch_tensormap(&tmX);
         ptx::prefetch_tensormap(&tmW);
+        if constexpr (GATED) ptx::prefetch_tensormap(&tmU);
         for (int s = 0; s < STAGES; ++s) {
             ptx::mbar_init(full_bar(s), 1);
             ptx::mbar_init(empty_bar(s), 1);
@@ -131,9 +142,9 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
 
     constexpr int TW = Cfg::TW;
     const int row0 = (warp >> 2) * TW;                // promotion warps: first row of C of this thread
-    unsigned long long acc[TW / 2];                   // ... and its rows row0 + 2 i, row0 + 2 i + 1, one column
+    unsigned long long acc[NW * TW / 2];              // ... and its rows row0 + 2 i, row0 + 2 i + 1, one column (of each matrix)
 #pragma unroll
-    for (int i = 0; i < TW / 2; ++i) acc[i] = 0ull;
+    for (int i = 0; i < NW * TW / 2; ++i) acc[i] = 0ull;
     bool ok = true;
 
     if (warp == Cfg::PROMO_WARPS) {
@@ -148,7 +159,8 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                 // whole boxes are written and counted: columns >= N and rows >= M read as 0
                 ptx::mbar_arrive_expect_tx(full_bar(s), Cfg::STAGE_BYTES);
                 ptx::tma_load_2d(dst, &tmW, n0, kb * 128, full_bar(s));
-                ptx::tma_load_2d(dst + Cfg::W_BYTES, &tmX, 0, kb * 128, full_bar(s));
+                if constexpr (GATED) ptx::tma_load_2d(dst + Cfg::W_BYTES, &tmU, n0, kb * 128, full_bar(s));
+                ptx::tma_load_2d(dst + NW * Cfg::W_BYTES, &tmX, 0, kb * 128, full_bar(s));
                 if (++s == STAGES) { s = 0; ph ^= 1u; }
             }
             if (!ok) {
@@ -174,13 +186,16 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                 if (!ok) break;
                 ptx::tc_fence_after_sync();
                 const uint32_t w_addr = stage_base + s * Cfg::STAGE_BYTES;
-                const uint64_t wdesc = ptx::make_smem_desc_sw128(w_addr, Cfg::W_BYTES, 1024);
-                const uint64_t xdesc = ptx::make_smem_desc(w_addr + Cfg::W_BYTES, Cfg::X_BYTES, x_atom, x_swizzle);
-                const uint32_t d = tmem_base + static_cast<uint32_t>(b * T);
+                const uint64_t xdesc = ptx::make_smem_desc(w_addr + NW * Cfg::W_BYTES, Cfg::X_BYTES, x_atom, x_swizzle);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)           // K = 32 per instruction = 4 swizzle atoms of 8 k-rows
-                    ptx::mma_f8f6f4(d, wdesc + static_cast<uint64_t>(j * (4096 >> 4)),
-                                    xdesc + static_cast<uint64_t>(j * ((4 * x_atom) >> 4)), idesc, j > 0 ? 1u : 0u);
+                for (int w = 0; w < NW; ++w) {
+                    const uint64_t wdesc = ptx::make_smem_desc_sw128(w_addr + w * Cfg::W_BYTES, Cfg::W_BYTES, 1024);
+                    const uint32_t d = tmem_base + static_cast<uint32_t>((b * NW + w) * T);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)       // K = 32 per instruction = 4 swizzle atoms of 8 k-rows
+                        ptx::mma_f8f6f4(d, wdesc + static_cast<uint64_t>(j * (4096 >> 4)),
+                                        xdesc + static_cast<uint64_t>(j * ((4 * x_atom) >> 4)), idesc, j > 0 ? 1u : 0u);
+                }
                 ptx::mma_commit(tfull_bar(b));
                 ptx::mma_commit(empty_bar(s));
                 if (++s == STAGES) { s = 0; ph ^= 1u; }
@@ -190,7 +205,7 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     } else if (warp == Cfg::PROMO_WARPS + 2) {
         // ---------------------------------------------------- scale products -------
         // a_scale[m, kb] * b_scale[n / 128, kb]: the tile's 128 columns touch at most two blocks of b_scale, one per 64
-        // columns.  Same hand-over and order of waits as in gemm_kernel.cuh.
+        // columns (gated: to one of each matrix, and `half` is the matrix).  Same hand-over and order of waits as in gemm_kernel.cuh.
         constexpr int AHEAD = 4, NA = T < 32 ? 1 : T / 32;
         float av[AHEAD][NA], bv[AHEAD][2];
         int nb[2];
@@ -207,7 +222,8 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                     a[i] = m < p.M ? __ldg(p.a_scale + static_cast<size_t>(fkb) * p.M + m) : 0.0f;
                 }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) b[h] = __ldg(p.b_scale + static_cast<size_t>(fkb) * p.sn + nb[h]) * p.elem_scale;
+                for (int h = 0; h < 2; ++h)
+                    b[h] = __ldg((GATED && h ? p.epi.up_scale : p.b_scale) + static_cast<size_t>(fkb) * p.sn + nb[GATED ? 0 : h]) * p.elem_scale;
             }
             ++fkb;
         };
@@ -242,7 +258,7 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
         }
     } else {
         // ---------------------------------------------------- promotion -------------
-        const uint32_t my_slot = slot_base + static_cast<uint32_t>((((warp >> 1) & 1) * T + row0) * 4);   // [column half][row]
+        const uint32_t my_slot = slot_base + static_cast<uint32_t>(((GATED ? 0 : (warp >> 1) & 1) * T + row0) * 4);   // [column half][row]
         const uint32_t my_tmem = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + static_cast<uint32_t>(row0);
         uint32_t item = 0;
         for (int kb = kb0; kb < kb1; ++kb, ++item) {
@@ -251,16 +267,20 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             ptx::tc_fence_after_sync();
-            const uint32_t sa = my_slot + (item % Cfg::SSLOTS) * (Cfg::SSLOT_FLOATS * 4);
-            uint32_t v[TW];
-            if constexpr (TW == 16) tmem_ld_x16_sync(my_tmem + static_cast<uint32_t>(b * T), v);
-            else tmem_ld_x32_sync(my_tmem + static_cast<uint32_t>(b * T), v);
 #pragma unroll
-            for (int i = 0; i < TW / 4; ++i) {
-                unsigned long long s0, s1;            // products of rows 4 i .. 4 i + 3
-                ptx::ld_shared_v2_b64(sa + static_cast<uint32_t>(16 * i), s0, s1);
-                acc[2 * i] = ptx::fma_f32x2((static_cast<unsigned long long>(v[4 * i + 1]) << 32) | v[4 * i], s0, acc[2 * i]);
-                acc[2 * i + 1] = ptx::fma_f32x2((static_cast<unsigned long long>(v[4 * i + 3]) << 32) | v[4 * i + 2], s1, acc[2 * i + 1]);
+            for (int w = 0; w < NW; ++w) {
+                const uint32_t sa = my_slot + (item % Cfg::SSLOTS) * (Cfg::SSLOT_FLOATS * 4) + static_cast<uint32_t>(w * T * 4);
+                uint32_t v[TW];
+                if constexpr (TW == 16) tmem_ld_x16_sync(my_tmem + static_cast<uint32_t>((b * NW + w) * T), v);
+                else tmem_ld_x32_sync(my_tmem + static_cast<uint32_t>((b * NW + w) * T), v);
+                unsigned long long* const mine = acc + w * (TW / 2);
+#pragma unroll
+                for (int i = 0; i < TW / 4; ++i) {
+                    unsigned long long s0, s1;        // products of rows 4 i .. 4 i + 3
+                    ptx::ld_shared_v2_b64(sa + static_cast<uint32_t>(16 * i), s0, s1);
+                    mine[2 * i] = ptx::fma_f32x2((static_cast<unsigned long long>(v[4 * i + 1]) << 32) | v[4 * i], s0, mine[2 * i]);
+                    mine[2 * i + 1] = ptx::fma_f32x2((static_cast<unsigned long long>(v[4 * i + 3]) << 32) | v[4 * i + 2], s1, mine[2 * i + 1]);
+                }
             }
             ptx::tc_fence_before_sync();
             __syncwarp();
@@ -269,27 +289,50 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     }
 
     // ---------------------------------------------------------------- result -------
-    if (S == 1) {
+    // The accumulator of row t (of this thread's TW) of matrix w, as a number.
+    auto sum_of = [&](int w, int t) { return t & 1 ? f32x2_hi(acc[w * (TW / 2) + t / 2]) : f32x2_lo(acc[w * (TW / 2) + t / 2]); };
+    if (!GATED && S == 1) {
         // straight from the registers (through shared memory, for wider stores, it took 0.6 us longer)
         const int n = n0 + (warp & 3) * 32 + lane;
         if (warp < Cfg::PROMO_WARPS && ok && n < p.N) {
+            if constexpr (EPI == EPI_BIAS_ACT) {
+                const float bias = p.epi.bias ? bias_1(p.epi, n) : 0.0f;
+                with_activation(p.epi, [&](auto act) {
 #pragma unroll
-            for (int t = 0; t < TW; ++t)
-                if (row0 + t < p.M)
-                    p.C[static_cast<size_t>(row0 + t) * p.N + n] = __float2bfloat16_rn(t & 1 ? f32x2_hi(acc[t / 2]) : f32x2_lo(acc[t / 2]));
+                    for (int t0 = 0; t0 < TW; t0 += 8) {               // eight residuals in flight
+                        float r[8];
+#pragma unroll
+                        for (int t = 0; t < 8; ++t)
+                            r[t] = p.epi.residual && row0 + t0 + t < p.rows ? __bfloat162float(p.epi.residual[(row0 + t0 + t) * p.epi.ldr + n]) : 0.0f;
+#pragma unroll
+                        for (int t = 0; t < 8; ++t)
+                            if (row0 + t0 + t < p.rows)
+                                p.C[static_cast<size_t>(row0 + t0 + t) * p.N + n] =
+                                    __float2bfloat16_rn(activate<decltype(act)::value>(sum_of(0, t0 + t) + bias, p.epi) + r[t]);
+                    }
+                });
+            } else {
+#pragma unroll
+                for (int t = 0; t < TW; ++t)
+                    if (row0 + t < p.rows) p.C[static_cast<size_t>(row0 + t) * p.N + n] = __float2bfloat16_rn(sum_of(0, t));
+            }
         }
     } else {
-        // partial sums to the CTA that finishes a row: [split][row of C][column] in its shared memory
+        // partial sums to the CTA that finishes a row: [split][row of C][matrix][column] in its shared memory
+        constexpr int PITCH = 512 * NW;               // bytes of a row
         const int per = (p.M + S - 1) / S;            // rows of C each CTA finishes
-        ptx::cluster_wait();                          // every CTA of the cluster runs
+        if (S > 1) ptx::cluster_wait();               // every CTA of the cluster runs
         if (warp < Cfg::PROMO_WARPS && ok) {
-            const uint32_t mine = red_base + static_cast<uint32_t>((rank * per * 128 + (warp & 3) * 32 + lane) * 4);
+            const uint32_t mine = red_base + static_cast<uint32_t>(rank * per * PITCH + ((warp & 3) * 32 + lane) * 4);
             int owner = row0 / per, local = row0 - owner * per;
+            // (a CTA's own address is one of its cluster's, of one CTA too)
             uint32_t dst = ptx::mapa(mine, static_cast<uint32_t>(owner < S ? owner : 0));
 #pragma unroll
             for (int t = 0; t < TW; ++t)
                 if (row0 + t < p.M) {
-                    ptx::st_shared_cluster_f32(dst + static_cast<uint32_t>(local * 512), t & 1 ? f32x2_hi(acc[t / 2]) : f32x2_lo(acc[t / 2]));
+#pragma unroll
+                    for (int w = 0; w < NW; ++w)
+                        ptx::st_shared_cluster_f32(dst + static_cast<uint32_t>(local * PITCH + w * 512), sum_of(w, t));
                     if (++local == per) {
                         local = 0;
                         ++owner;
@@ -297,22 +340,48 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                     }
                 }
         }
-        ptx::cluster_sync();
+        if (S > 1) ptx::cluster_sync();
+        else __syncthreads();
         if (*abort_flag == 0u) {
             const int t0 = rank * per, rows = t0 + per < p.M ? per : p.M - t0;
             // four columns of one row per thread and round, all splits' loads in flight together
             for (int idx = static_cast<int>(threadIdx.x); idx < rows * 32; idx += Cfg::THREADS) {
                 const int t = idx >> 5, c = (idx & 31) * 4;
-                const float4* src = reinterpret_cast<const float4*>(red_ptr + t * 128 + c);
-                float4 v[8];
+                auto sum_at = [&](int w) {
+                    const float4* src = reinterpret_cast<const float4*>(red_ptr + (t * NW + w) * 128 + c);
+                    float4 v[8];
 #pragma unroll
-                for (int s = 0; s < 8; ++s)
-                    if (s < S) v[s] = src[static_cast<size_t>(s) * per * 32];
-                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int s = 0; s < 8; ++s)
+                        if (s < S) v[s] = src[static_cast<size_t>(s) * per * (32 * NW)];
+                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                for (int s = 0; s < 8; ++s)           // split order
-                    if (s < S) { sum.x += v[s].x; sum.y += v[s].y; sum.z += v[s].z; sum.w += v[s].w; }
-                if (n0 + c < p.N) {
+                    for (int s = 0; s < 8; ++s)       // split order
+                        if (s < S) { sum.x += v[s].x; sum.y += v[s].y; sum.z += v[s].z; sum.w += v[s].w; }
+                    return sum;
+                };
+                float4 sum = sum_at(0);
+                if constexpr (GATED) {
+                    const float4 up = sum_at(1);
+                    with_activation(p.epi, [&](auto act) {
+                        constexpr int A = decltype(act)::value;
+                        sum = make_float4(activate<A>(sum.x, p.epi) * up.x, activate<A>(sum.y, p.epi) * up.y, activate<A>(sum.z, p.epi) * up.z,
+                                          activate<A>(sum.w, p.epi) * up.w);
+                    });
+                }
+                if constexpr (EPI == EPI_GATED_FP8) {
+                    // a warp's lanes are the 128 columns of row t
+                    const float amax = warp_absmax_nan(max_nan(max_nan(fabsf(sum.x), fabsf(sum.y)), max_nan(fabsf(sum.z), fabsf(sum.w))));
+                    float inverse;
+                    const float f = scale_factor(amax, p.epi.fp8_max, inverse);
+                    if ((idx & 31) == 0) p.epi.scale_out[static_cast<size_t>(n0 >> 7) * p.M + t0 + t] = inverse;
+                    const uint32_t lo = cvt_e4m3x2(sum.x * f, sum.y * f), hi = cvt_e4m3x2(sum.z * f, sum.w * f);
+                    uint8_t* dst = p.epi.q_out + static_cast<size_t>(n0 + c) * p.M + t0 + t;
+                    dst[0] = static_cast<uint8_t>(lo);
+                    dst[p.M] = static_cast<uint8_t>(lo >> 8);
+                    dst[2 * p.M] = static_cast<uint8_t>(hi);
+                    dst[3 * p.M] = static_cast<uint8_t>(hi >> 8);
+                } else if (n0 + c < p.N && t0 + t < p.rows) {
+                    if constexpr (EPI == EPI_BIAS_ACT) sum = finish_4(sum, p.epi, t0 + t, n0 + c);
                     uint2 q;
                     q.x = pack_bf16x2(sum.x, sum.y);
                     q.y = pack_bf16x2(sum.z, sum.w);

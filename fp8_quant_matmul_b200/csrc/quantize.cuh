@@ -27,20 +27,13 @@
 // The conversion is the hardware's cvt.rn.satfinite.e4m3x2.f32 (round to nearest even; the clamp before it keeps
 // every value inside the format's range, where it equals torch's cast bit for bit).
 #pragma once
+#include "epilogue.cuh"
 #include <cuda_bf16.h>
 #include <cstdint>
 
 namespace fp8bs {
 
 __host__ __device__ inline uint8_t float_to_e4m3fn_rne(float x);   // defined in fp8bs.cu
-
-// Two fp32 -> two e4m3fn bytes (lo in bits 0-7, hi in bits 8-15), round to nearest even.
-__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi)
-{
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 
 constexpr int QUANTIZE_PITCH = 132;                                // words per row group: 128 k + 4 (16-byte aligned rows)
 constexpr int QUANTIZE_TILE_WORDS = 32 * QUANTIZE_PITCH;           // [row group of 4][k]: one word = 4 rows at one k

@@ -46,21 +46,6 @@ struct NormParams {
     float inv_K, eps, fp8_max;
 };
 
-// torch's maximum: NaN if either is (fmaxf drops it), so that a NaN in a row shows in its bytes and scales.
-__device__ __forceinline__ float max_nan(float a, float b)
-{
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-// The largest magnitude over a warp's lanes, NaN if one is.
-__device__ __forceinline__ float warp_absmax_nan(float a)
-{
-    float d;
-    asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(a));
-    return d;
-}
-
 // Adds up 16 values per lane, one per row, over the 32 lanes: the halving butterfly of quantize.cuh (16 shuffles).  Lanes 2 r and
 // 2 r + 1 return row r's.
 __device__ __forceinline__ float sum_16_rows(const float (&a)[16], int lane)

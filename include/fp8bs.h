@@ -135,6 +135,38 @@ int fp8bs_gemm_ex(const void* A, const void* B, const float* a_scale, const floa
                   int M, int N, int K, int n0, int n_total, int path, int splits, int tile_n,
                   void* workspace, size_t workspace_bytes, void* stream);
 
+/* The operator with an epilogue:  C = round(act(sum + bias) + residual), everything in fp32 until the one rounding to bf16, sum being
+ * what fp8bs_gemm rounds.  M, N, K and the operands as there; of the M rows the first `rows` (1..M) exist in C and in the residual:
+ * nothing is written behind them, so that a call for one token (A padded to 16 rows) has a C of one row.
+ *   bias        [N], bf16 (bias_is_bf16 != 0) or fp32, 16-byte aligned; NULL: none
+ *   activation  FP8BS_ACT_*
+ *   residual    [rows, N] bf16 with a row pitch of ld_residual elements (>= N, a multiple of 8), 16-byte aligned; NULL: none.  It may be
+ *               C itself (ld_residual = N); it must not overlap C otherwise.
+ *   splits      0 = let the library choose; 1..8 = K cut over a cluster of that many CTAs
+ *   tile_n      0 = choose; 128; 256 (splits 0 or > 1); 256 | FP8BS_TILE_PAIR (splits 0 or 1); FP8BS_SMALL_M (M <= 64)
+ * Needs no workspace.  Asynchronous on `stream`. */
+#define FP8BS_ACT_NONE      0   /* x */
+#define FP8BS_ACT_RELU      1   /* max(x, 0) */
+#define FP8BS_ACT_SILU      2   /* x / (1 + exp(-x)) */
+#define FP8BS_ACT_GELU      3   /* x (1 + erf(x / sqrt 2)) / 2 */
+#define FP8BS_ACT_GELU_TANH 4   /* x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */
+int fp8bs_gemm_bias_act(const void* A, const void* B, const float* a_scale, const float* b_scale, void* C, int M, int N, int K, int rows,
+                        const void* bias, int bias_is_bf16, int activation, const void* residual, long long ld_residual, int splits,
+                        int tile_n, void* stream);
+
+/* Both projections of a gated feed-forward layer, its activation and product, one launch:
+ *     h = act(A . B_gate) * (A . B_up), each product scaled as in the operator, everything in fp32 until the one rounding
+ * B_gate, B_up: N x K column-major; gate_scale, up_scale: [ceil(N/128), K/128] as b_scale.
+ *   h_scale NULL      H is bf16 [rows, N]: the first `rows` (1..M) of the M rows
+ *   h_scale non-NULL  h leaves in 8 bits as the next product's A (its K is this N, a multiple of 128): H[m + M*n] e4m3fn bytes and
+ *                     h_scale[m + M*(n/128)], scaled per row and 128 columns as by fp8bs_quantize_rowwise, with fp8_max as there.  All M rows
+ *                     are written (rows of zeros in A become zeros); `rows` is not looked at beyond 1..M
+ *   activation        FP8BS_ACT_*;   splits, tile_n as above: 256 or 256 | FP8BS_TILE_PAIR (128 columns of both products) or FP8BS_SMALL_M
+ * Needs no workspace.  Asynchronous on `stream`. */
+int fp8bs_gemm_gated(const void* A, const void* B_gate, const void* B_up, const float* a_scale, const float* gate_scale, const float* up_scale,
+                     void* H, float* h_scale, int M, int N, int K, int rows, int activation, float fp8_max, int splits, int tile_n,
+                     void* stream);
+
 /* One thread per C element, scalar fp32: the reference's ground-truth kernel restated in
  * CUDA (ref_kernel, check.cu:30-49; gemmGPU option 2, check.cu:87-90).  Slow; for the
  * on-device cross-check of the `check` program. */
