@@ -334,17 +334,23 @@ def gemm(A, B, a_scale, b_scale, C=None, M=None, N=None, K=None, path=PATH_AUTO,
     return C
 
 
-def _check_operands(index, M, N, K, rows, activation, pairs):
-    """What the fused calls check before pointers are handed over; returns the activation's number."""
+def _fits(t, index, n, size):
+    return t.get_device() == index and t.is_contiguous() and t.numel() >= n and t.element_size() == size
+
+
+def _check_fused(index, M, N, K, rows, activation, A, a_scale, weights):
+    """What the fused calls check before pointers are handed over; returns the activation's number.  weights: matrices and their scales."""
     if M is None or N is None or K is None:
         raise ValueError("M, N, K are required (operands are flat column-major buffers)")
     if not 1 <= rows <= M:
         raise ValueError("rows has to be in 1..M")
-    for name, t, n, kind in pairs:
-        if t.get_device() != index or not t.is_contiguous():
-            raise ValueError("%s has to be a contiguous tensor on A's device" % name)
-        if t.numel() < n or t.element_size() != kind:
-            raise ValueError("%s has to hold %d elements of %d bytes" % (name, n, kind))
+    blocks = K // 128
+    good = _fits(A, index, M * K, 1) and _fits(a_scale, index, M * blocks, 4)
+    for B, scale in weights:
+        good = good and _fits(B, index, N * K, 1) and _fits(scale, index, (N + 127) // 128 * blocks, 4)
+    if not good:
+        raise ValueError("operands have to be contiguous tensors on A's device: 1-byte elements of M*K and N*K, fp32 scales of M*K/128 and "
+                         "ceil(N/128)*K/128")
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError("activation has to be one of " + ", ".join(ACTIVATIONS))
@@ -352,7 +358,7 @@ def _check_operands(index, M, N, K, rows, activation, pairs):
 
 
 def _check_out(t, rows, N, dtype, index, name):
-    if tuple(t.shape) != (rows, N) or t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+    if t.shape != (rows, N) or t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
         raise ValueError("%s has to be a contiguous %s tensor [rows, N] on A's device" % (name, dtype))
 
 
@@ -369,17 +375,15 @@ def gemm_bias_act(A, B, a_scale, b_scale, C=None, M=None, N=None, K=None, bias=N
         raise RuntimeError("fp8bs.gemm_bias_act needs CUDA tensors; there is no CPU implementation")
     index = A.get_device()
     rows = M if rows is None else rows
-    act = _check_operands(index, M, N, K, rows, activation,
-                          (("A", A, M * K, 1), ("B", B, N * K, 1), ("a_scale", a_scale, M * (K // 128), 4),
-                           ("b_scale", b_scale, -(-N // 128) * (K // 128), 4)) if M is not None and N is not None and K is not None else ())
+    act = _check_fused(index, M, N, K, rows, activation, A, a_scale, ((B, b_scale),))
     bias_ptr, bias_bf16, r_ptr, ldr = None, 0, None, N
     if bias is not None:
         bias_bf16 = _is_bf16(bias.dtype, "bias")
-        if tuple(bias.shape) != (N,) or bias.get_device() != index or not bias.is_contiguous():
+        if bias.shape != (N,) or bias.get_device() != index or not bias.is_contiguous():
             raise ValueError("bias has to be a contiguous tensor [N] on A's device")
         bias_ptr = bias.data_ptr()
     if residual is not None:
-        if (tuple(residual.shape) != (rows, N) or residual.dtype is not torch.bfloat16 or residual.get_device() != index
+        if (residual.shape != (rows, N) or residual.dtype is not torch.bfloat16 or residual.get_device() != index
                 or residual.stride(1) != 1):
             raise ValueError("residual has to be a bf16 tensor [rows, N] on A's device with contiguous rows")
         r_ptr = residual.data_ptr()
@@ -405,11 +409,7 @@ def gemm_gated(A, B_gate, B_up, a_scale, gate_scale, up_scale, M=None, N=None, K
         raise RuntimeError("fp8bs.gemm_gated needs CUDA tensors; there is no CPU implementation")
     index = A.get_device()
     rows = M if rows is None else rows
-    known = M is not None and N is not None and K is not None
-    n_scales = -(-N // 128) * (K // 128) if known else 0
-    act = _check_operands(index, M, N, K, rows, activation,
-                          (("A", A, M * K, 1), ("B_gate", B_gate, N * K, 1), ("B_up", B_up, N * K, 1), ("a_scale", a_scale, M * (K // 128), 4),
-                           ("gate_scale", gate_scale, n_scales, 4), ("up_scale", up_scale, n_scales, 4)) if known else ())
+    act = _check_fused(index, M, N, K, rows, activation, A, a_scale, ((B_gate, gate_scale), (B_up, up_scale)))
     s_ptr = scales = None
     if quantize:
         if H is not None:
@@ -503,7 +503,7 @@ def _call(name, index, *args):
     """A library call for tensors of CUDA device `index`, on that device's current stream."""
     torch = _torch()
     fn = getattr(lib(), name)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, _stream(index))
     else:                                           # the library launches on the current device
         with torch.cuda.device(index):
@@ -513,12 +513,13 @@ def _call(name, index, *args):
 
 
 def _is_bf16(dtype, what):
+    """The flag the library takes for fp32 or bf16."""
     torch = _torch()
     if dtype is torch.bfloat16:
         return 1
-    if dtype is torch.float32:
-        return 0
-    raise ValueError("%s has to be fp32 or bf16" % what)
+    if dtype is not torch.float32:
+        raise ValueError("%s has to be fp32 or bf16" % what)
+    return 0
 
 
 def rmsnorm_quantize(X, weight, residual=None, eps=1e-6, fp8_max=448.0, residual_out=None):
@@ -531,33 +532,33 @@ def rmsnorm_quantize(X, weight, residual=None, eps=1e-6, fp8_max=448.0, residual
     X, residual and weight: fp32 or bf16 each.  X and residual may be column slices (any row stride of whole 16 bytes).
     """
     torch = _torch()
-    if not X.is_cuda or X.dim() != 2 or X.stride(1) != 1:
+    shape = X.shape
+    if not X.is_cuda or len(shape) != 2 or X.stride(1) != 1:
         raise ValueError("X has to be a 2-D CUDA tensor [rows, K] with contiguous rows")
-    rows, K = X.shape
+    rows, K = shape
     index = X.get_device()
     if weight.shape != (K,) or weight.get_device() != index or not weight.is_contiguous():
         raise ValueError("weight has to be a contiguous tensor [K] on X's device")
-    x_bf16, w_bf16, r_bf16 = _is_bf16(X.dtype, "X"), _is_bf16(weight.dtype, "weight"), 0
-    r_ptr = out_ptr = None
-    ldr = K
+    r_bf16, r_ptr, out_ptr, ldr = 0, None, None, K
     if residual is not None:
-        if residual.shape != X.shape or residual.get_device() != index or residual.stride(1) != 1:
+        if residual.shape != shape or residual.get_device() != index or residual.stride(1) != 1:
             raise ValueError("residual has to be a tensor like X, on its device, with contiguous rows")
         r_bf16 = _is_bf16(residual.dtype, "residual")
         if residual_out is None:
-            residual_out = torch.empty((rows, K), dtype=residual.dtype, device=X.device)
-        elif (residual_out.shape != X.shape or residual_out.dtype is not residual.dtype or residual_out.get_device() != index
+            residual_out = residual.new_empty(shape)
+        elif (residual_out.shape != shape or residual_out.dtype is not residual.dtype or residual_out.get_device() != index
               or not residual_out.is_contiguous()):
             raise ValueError("residual_out has to be a contiguous tensor [rows, K] of the residual's type on X's device")
         r_ptr, out_ptr = residual.data_ptr(), residual_out.data_ptr()
-        ldr = residual.stride(0) if rows > 1 else K
+        if rows > 1:
+            ldr = residual.stride(0)
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
     M = (rows + 15) // 16 * 16
-    q = torch.empty(M * K, dtype=torch.uint8, device=X.device)
-    scales = torch.empty(M * (K // 128), dtype=torch.float32, device=X.device)
-    _call("fp8bs_rmsnorm_quantize", index, X.data_ptr(), x_bf16, X.stride(0) if rows > 1 else K, r_ptr, r_bf16, ldr, out_ptr,
-          weight.data_ptr(), w_bf16, q.data_ptr(), scales.data_ptr(), rows, K, eps, fp8_max)
+    q = X.new_empty(M * K, dtype=torch.uint8)
+    scales = X.new_empty(M * (K // 128), dtype=torch.float32)
+    _call("fp8bs_rmsnorm_quantize", index, X.data_ptr(), _is_bf16(X.dtype, "X"), X.stride(0) if rows > 1 else K, r_ptr, r_bf16, ldr, out_ptr,
+          weight.data_ptr(), _is_bf16(weight.dtype, "weight"), q.data_ptr(), scales.data_ptr(), rows, K, eps, fp8_max)
     return (q, scales) if residual is None else (q, scales, residual_out)
 
 

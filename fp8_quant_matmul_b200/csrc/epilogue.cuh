@@ -2,9 +2,12 @@
 //   none   x                     silu       x / (1 + exp(-x))
 //   relu   x < 0 ? 0 : x         gelu       x (1 + erf(x / sqrt 2)) / 2
 //                                gelu_tanh  x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) / 2 = x / (1 + exp(-2 sqrt(2/pi) (x + 0.044715 x^3)))
-// silu and gelu_tanh are one function with two constants, x / (1 + 2^(x (a + b x^2))): an exponential and a reciprocal of the
-// special-function unit per element.  Their errors (2^-22 each, and the argument's rounding) are below 1 % of a bf16 step where the
-// result is not itself negligible, and an output in 8 bits has its scale from the largest elements, where 2^(..) is next to nothing.
+// silu and gelu_tanh are one function with two constants, x / (1 + 2^(x (a + b x^2))).  The special-function unit (four lanes per clock and
+// scheduler) is what activations cost: two values share one reciprocal (1 / d0 = d1 / (d0 d1)), 1.5 operations of that unit per value
+// instead of 2.  Errors (2^-22 of the exponential and of the reciprocal, and the argument's rounding) are below 1 % of a bf16 step where
+// the result is not itself negligible, and an output in 8 bits has its scale from the largest elements, where 2^(..) is next to nothing.
+// (In packed fp32 instructions the activations were no faster and the K loop of the pair kernel, which shares their registers, 17 %
+// slower, whichever was chosen at run time.)
 #pragma once
 #include "ptx.cuh"
 #include <cuda_bf16.h>
@@ -46,38 +49,66 @@ struct Epilogue {
     float* scale_out;               // ... and its inverse scales [N / 128][M]
     int bias_is_bf16;
     int act;
-    float a, b;                     // ACT_LOGISTIC, log2 e included
+    float a, b, lowest;             // ACT_LOGISTIC: the constants, log2 e included; below `lowest` the function is -1e-16 at most
     float fp8_max;
 };
 
-__device__ __forceinline__ float logistic_times(float x, float a, float b)
+// Two fp32 values in one 64-bit register, the operand form of fma.rn.f32x2 (low word = first value).
+__device__ __forceinline__ unsigned long long pack_f32x2(float lo, float hi)
 {
-    // The square is held finite, so that b = 0 leaves a and not 0 * infinity.
-    const float z = x * fmaf(b, fminf(x * x, 1e30f), a);
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    return x * r;
+    return static_cast<unsigned long long>(__float_as_uint(lo)) | (static_cast<unsigned long long>(__float_as_uint(hi)) << 32);
 }
+__device__ __forceinline__ float f32x2_lo(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float f32x2_hi(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+
+__device__ __forceinline__ float ex2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_approx(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// x / (1 + 2^(x (a + b x^2))).  The argument of the exponential is held in a range (2^-6700 .. 2^60) in which nothing overflows and a NaN does not
+// reach the other value of the pair; the factor x keeps NaN and +infinity.
+__device__ __forceinline__ unsigned long long logistic_times_2(unsigned long long x, const Epilogue& e)
+{
+    const float x0 = max_nan(f32x2_lo(x), e.lowest), x1 = max_nan(f32x2_hi(x), e.lowest);
+    const float t0 = fminf(x0, 40.0f), t1 = fminf(x1, 40.0f);
+    const float d0 = 1.0f + ex2_approx(t0 * fmaf(t0 * t0, e.b, e.a)), d1 = 1.0f + ex2_approx(t1 * fmaf(t1 * t1, e.b, e.a));
+    const float r = rcp_approx(d0 * d1);
+    return pack_f32x2(x0 * (r * d1), x1 * (r * d0));
+}
+
 // x (1 + erf(x / sqrt 2)) / 2 = max(x, 0) - |x| erfc(|x| / sqrt 2) / 2 with erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), t = 1 / (1 + p z): formula
 // 7.1.26 of Abramowitz and Stegun, off by 1.5e-7 at most, that is 7.5e-8 |x| here; and the tail below 0 has no cancellation.  (CUDA's
 // erff in this place cost the K loop of the pair kernel 15 spilled registers.)
-__device__ __forceinline__ float erf_times(float x)
+__device__ __forceinline__ unsigned long long erf_times_2(unsigned long long x)
 {
-    const float ax = fminf(fabsf(x), 100.0f);                        // the tail is 0 there; infinity would be 0 * infinity
-    const float z = ax * 0.70710678118654752f;
-    float t, e;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f, z, 1.0f)));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * z * -1.4426950408889634f));
-    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    return (x < 0.0f ? 0.0f : x) - 0.5f * ax * poly * e;             // a NaN stays one
+    const float x0 = f32x2_lo(x), x1 = f32x2_hi(x);
+    const float a0 = fminf(fabsf(x0), 100.0f), a1 = fminf(fabsf(x1), 100.0f);       // the tail is 0 there; NaN becomes 100
+    const float z0 = a0 * 0.70710678118654752f, z1 = a1 * 0.70710678118654752f;
+    const float p0 = fmaf(0.3275911f, z0, 1.0f), p1 = fmaf(0.3275911f, z1, 1.0f), r = rcp_approx(p0 * p1);
+    auto tail = [](float t, float z) {
+        const float poly = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+        return poly * t * ex2_approx(z * -1.4426950408889634f * z);
+    };
+    const float c0 = tail(r * p1, z0), c1 = tail(r * p0, z1);
+    // max(x, 0) keeps a NaN
+    return pack_f32x2(fmaf(a0 * -0.5f, c0, x0 < 0.0f ? 0.0f : x0), fmaf(a1 * -0.5f, c1, x1 < 0.0f ? 0.0f : x1));
 }
 template <int ACT>
-__device__ __forceinline__ float activate(float x, const Epilogue& e)
+__device__ __forceinline__ unsigned long long activate_2(unsigned long long x, const Epilogue& e)
 {
-    if constexpr (ACT == ACT_RELU) return x < 0.0f ? 0.0f : x;       // a NaN stays one
-    else if constexpr (ACT == ACT_LOGISTIC) return logistic_times(x, e.a, e.b);
-    else if constexpr (ACT == ACT_ERF) return erf_times(x);
+    if constexpr (ACT == ACT_RELU)                                   // a NaN stays one
+        return pack_f32x2(f32x2_lo(x) < 0.0f ? 0.0f : f32x2_lo(x), f32x2_hi(x) < 0.0f ? 0.0f : f32x2_hi(x));
+    else if constexpr (ACT == ACT_LOGISTIC) return logistic_times_2(x, e);
+    else if constexpr (ACT == ACT_ERF) return erf_times_2(x);
     else return x;
 }
 // f(integral constant of the activation): one branch per call of this, not per element.
@@ -105,6 +136,22 @@ __device__ __forceinline__ float bias_1(const Epilogue& e, int n)
     return e.bias_is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[n]) : __ldg(static_cast<const float*>(e.bias) + n);
 }
 
+__device__ __forceinline__ float4 activate_4(float4 v, const Epilogue& e)
+{
+    unsigned long long a = pack_f32x2(v.x, v.y), b = pack_f32x2(v.z, v.w);
+    with_activation(e, [&](auto act) {
+        a = activate_2<decltype(act)::value>(a, e);
+        b = activate_2<decltype(act)::value>(b, e);
+    });
+    return make_float4(f32x2_lo(a), f32x2_hi(a), f32x2_lo(b), f32x2_hi(b));
+}
+// act(gate) * up
+__device__ __forceinline__ float4 gate_4(float4 gate, float4 up, const Epilogue& e)
+{
+    const float4 g = activate_4(gate, e);
+    return make_float4(g.x * up.x, g.y * up.y, g.z * up.z, g.w * up.w);
+}
+
 // act(v + bias) + residual of four neighbouring columns of row m.
 __device__ __forceinline__ float4 finish_4(float4 v, const Epilogue& e, int m, int n)
 {
@@ -114,10 +161,7 @@ __device__ __forceinline__ float4 finish_4(float4 v, const Epilogue& e, int m, i
         const float4 b = bias_4(e, n);
         v = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
     }
-    with_activation(e, [&](auto act) {
-        constexpr int A = decltype(act)::value;
-        v = make_float4(activate<A>(v.x, e), activate<A>(v.y, e), activate<A>(v.z, e), activate<A>(v.w, e));
-    });
+    v = activate_4(v, e);
     if (e.residual)
         v = make_float4(v.x + __uint_as_float(r.x << 16), v.y + __uint_as_float(r.x & 0xffff0000u), v.z + __uint_as_float(r.y << 16),
                         v.w + __uint_as_float(r.y & 0xffff0000u));

@@ -269,19 +269,31 @@ constexpr int SMALL_M_MAX = 64;
 // 9.5, .., 6.2 with 8; 32 x 4096 x 2048 (32 tiles) 9.9, 7.5, 6.7, 6.2.  Up to four K blocks the reduction costs more than it
 // saves: 16 x 4608 x 256 2.9, 3.6; 32 x 7168 x 512 4.5, 5.1.  With long K (16 K blocks per CTA and more) two CTAs per SM keep
 // more loads in flight: 16 x 7168 x 7168 16.0 with 2 splits, 14.0 with 4.
-// ctas_per_sm: 1 for the gated form, whose CTA keeps twice as many weights in flight.
-static Config small_m_config(const DeviceModel& dm, int N, int K, int splits, int ctas_per_sm = 2)
+static Config small_m_config(const DeviceModel& dm, int N, int K, int splits)
 {
     const int tiles = ceil_div(N, 128), KB = K / 128;
     int s = splits;
     if (s == 0) {
         s = KB <= 4 ? 1 : dm.sm_count / tiles;
-        if (ctas_per_sm > 1 && s >= 1 && KB / s >= 16 && 4 * tiles * s <= 7 * dm.sm_count) s *= 2;
+        if (s >= 1 && KB / s >= 16 && 4 * tiles * s <= 7 * dm.sm_count) s *= 2;
         if (s > MAX_CLUSTER_SPLITS) s = MAX_CLUSTER_SPLITS;
         if (s > KB) s = KB;
         while (s > 1 && dm.max_clusters[s] < 1) --s;
         if (s < 1) s = 1;
     }
+    return Config{s > 1 ? FP8BS_PATH_MN_SMALL : FP8BS_PATH_MN_LARGE, 128, s, 1, 5, 0};
+}
+
+// The gated form has one CTA per SM (its stages hold both matrices), so a cluster that does not fit beside the others waits for a whole
+// one: the most splits whose clusters all run at once.  16 rows, 1..8 splits: 2048 x 7168 (16 tiles) 27.7, 16.0, 12.4, 11.0, 10.4, 10.0 (22
+// clusters of 6 fit), 14.7, 14.8 (15 of 8); 4608 x 7168 (36 tiles) 25.6, 17.5, 16.0, 22.6; 7168 x 2304 (56) 14.0, 11.4, 15.2; 1024 x 2048 (8) 9.3,
+// 6.3, .., 4.4 with 8; 4096 x 512 (32) 6.2, 5.6, 5.7, 5.0.
+static Config gated_small_m_config(const DeviceModel& dm, int N, int K, int splits)
+{
+    const int tiles = ceil_div(N, 128), KB = K / 128;
+    int s = splits;
+    if (s == 0)
+        for (s = std::min(KB, MAX_CLUSTER_SPLITS); s > 1 && dm.max_clusters[s] < tiles; --s) {}
     return Config{s > 1 ? FP8BS_PATH_MN_SMALL : FP8BS_PATH_MN_LARGE, 128, s, 1, 5, 0};
 }
 
@@ -473,7 +485,7 @@ static int choose_fused(const DeviceModel& dm, int M, int N, int K, bool gated, 
     if (t != 0 && t != 128 && t != 256 && t != (256 | FP8BS_TILE_PAIR)) return FP8BS_ERR_ARG;
     if ((tile_n & FP8BS_SMALL_M) && (M > SMALL_M_MAX || (t != 0 && t != 128))) return FP8BS_ERR_ARG;
     if ((tile_n & FP8BS_SMALL_M) || (tile_n == 0 && M <= SMALL_M_MAX)) {
-        *out = small_m_config(dm, N, K, splits, gated ? 1 : 2);
+        *out = gated ? gated_small_m_config(dm, N, K, splits) : small_m_config(dm, N, K, splits);
         return FP8BS_OK;
     }
     double best_cost = 1e300;
@@ -922,9 +934,10 @@ static int fused_impl(const void* A, const void* B, const void* B2, const float*
     const double log2e = 1.4426950408889634, c = 2.0 * 0.7978845608028654;             // 2 sqrt(2 / pi)
     switch (activation) {
         case FP8BS_ACT_RELU: e.act = ACT_RELU; break;
-        case FP8BS_ACT_SILU: e.act = ACT_LOGISTIC; e.a = static_cast<float>(-log2e); e.b = 0.0f; break;
+        case FP8BS_ACT_SILU: e.act = ACT_LOGISTIC; e.a = static_cast<float>(-log2e); e.b = 0.0f; e.lowest = -40.0f; break;
         case FP8BS_ACT_GELU: e.act = ACT_ERF; break;
-        case FP8BS_ACT_GELU_TANH: e.act = ACT_LOGISTIC; e.a = static_cast<float>(-log2e * c); e.b = static_cast<float>(-log2e * c * 0.044715); break;
+        case FP8BS_ACT_GELU_TANH: e.act = ACT_LOGISTIC; e.a = static_cast<float>(-log2e * c); e.b = static_cast<float>(-log2e * c * 0.044715);
+            e.lowest = -7.4f; break;
         default: e.act = ACT_NONE;
     }
     if (!gated) return launch_bias_act(cfg, tm, p, dev->sm_count, st);

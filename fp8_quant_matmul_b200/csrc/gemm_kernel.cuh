@@ -232,14 +232,6 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, vola
     }
 }
 
-// Two fp32 values in one 64-bit register, the operand form of fma.rn.f32x2 (low word = first value).
-__device__ __forceinline__ unsigned long long pack_f32x2(float lo, float hi)
-{
-    return static_cast<unsigned long long>(__float_as_uint(lo)) | (static_cast<unsigned long long>(__float_as_uint(hi)) << 32);
-}
-__device__ __forceinline__ float f32x2_lo(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v)); }
-__device__ __forceinline__ float f32x2_hi(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
-
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi)
 {
     __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);  // .x = lo (low half), round to nearest even
@@ -319,14 +311,6 @@ __device__ __forceinline__ void stage_and_store_2x64(const CUtensorMap* tmC, int
     }
 }
 
-// 64 columns of this thread's row, two fp32 per register pair.
-typedef unsigned long long Cols64[2][16];
-
-template <class F>
-__device__ __forceinline__ unsigned long long each_f32(unsigned long long v, F f)
-{
-    return pack_f32x2(f(f32x2_lo(v)), f(f32x2_hi(v)));
-}
 // v = act(v + bias): bias from shared memory (64 fp32), or none.
 template <int ACT>
 __device__ __forceinline__ void bias_and_activate(unsigned long long (&v)[16], uint32_t bias_addr, bool has_bias, const Epilogue& e)
@@ -341,7 +325,7 @@ __device__ __forceinline__ void bias_and_activate(unsigned long long (&v)[16], u
         }
     if constexpr (ACT != ACT_NONE)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = each_f32(v[i], [&](float x) { return activate<ACT>(x, e); });
+        for (int i = 0; i < 16; ++i) v[i] = activate_2<ACT>(v[i], e);
 }
 // stage_64 onto the residual that lies in the box.
 __device__ __forceinline__ void add_and_stage_64(uint8_t* stg, int lane, const unsigned long long (&c0)[16], const unsigned long long (&c1)[16])
@@ -540,6 +524,84 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     // First column, within the tile, of the 64-column piece q of column group g.  A pair's MMA of part h takes 64 columns
     // from each CTA's B slab (slab r holds the tile's columns 128 r ..), which come out as the part's two pieces.
     auto col_of = [](int g, int q) { return CG == 2 ? g * 64 + q * 128 : g * Cfg::COLS + q * 64; };
+
+    // MODE 2: the cluster reduction.  Gated it runs inside the promotion warps' branch: its sums of two products would spill in the 64
+    // registers that the code after the branches has to make do with (and spills leave the SM: shared memory takes all of L1).  15 us.
+    auto cluster_meet = [&]() {
+        __syncthreads();                 // this CTA's partial tile is complete ...
+        ptx::cluster_sync();             // ... and so are those of the other K ranges of the tile
+    };
+    auto cluster_reduce = [&]() {
+        if (*abort_flag != 0u) return;
+        const int S = p.splits;
+        const int my = static_cast<int>(ptx::cluster_ctarank());     // = this CTA's split index
+        int tile, m0, n0, kb0, kb1;
+        decode(static_cast<int>(blockIdx.x), tile, m0, n0, kb0, kb1);
+        // the rows this CTA finishes (gated fp8: pairs of rows)
+        const int r0 = EPI == EPI_GATED_FP8 ? 2 * ((64 * my) / S) : (128 * my) / S;
+        const int r1 = EPI == EPI_GATED_FP8 ? 2 * ((64 * (my + 1)) / S) : (128 * (my + 1)) / S;
+        uint32_t peer[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) peer[s] = ptx::mapa(stage_base, static_cast<uint32_t>(s < S ? s : 0));
+        auto sum_at = [&](int row, int c) {                         // splits in fixed order: bit-deterministic
+            const uint32_t off = static_cast<uint32_t>(row * PART_PITCH + c * 4);
+            float4 v[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (s < S) v[s] = ptx::ld_shared_cluster_v4(peer[s] + off);
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (s < S) { sum.x += v[s].x; sum.y += v[s].y; sum.z += v[s].z; sum.w += v[s].w; }
+            return sum;
+        };
+        if constexpr (GATED) {
+            // A warp takes a row (fp8: two neighbouring ones, a 16-bit store per column), a lane four columns.  Partial tiles are laid
+            // out [column group][first | second][64].
+            constexpr int ROWS = EPI == EPI_GATED_FP8 ? 2 : 1;
+            const int c = lane * 4, part = (c >> 6) * 128 + (c & 63);
+            for (int row = r0 + (warp - 4) * ROWS; row < r1; row += Cfg::PROMO_WARPS * ROWS) {
+                uint32_t q[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 1
+                for (int i = 0; i < ROWS; ++i) {
+                    const float4 g = sum_at(row + i, part), up = sum_at(row + i, part + 64);
+                    const float4 h = gate_4(g, up, p.epi);
+                    const int m = m0 + row + i;
+                    if constexpr (EPI == EPI_GATED_FP8) {
+                        const float amax = warp_absmax_nan(max_nan(max_nan(fabsf(h.x), fabsf(h.y)), max_nan(fabsf(h.z), fabsf(h.w))));
+                        float inverse;
+                        const float f = scale_factor(amax, p.epi.fp8_max, inverse);
+                        if (lane == 0 && m < p.M) p.epi.scale_out[static_cast<size_t>(n0 >> 7) * p.M + m] = inverse;
+                        const uint32_t lo = cvt_e4m3x2(h.x * f, h.y * f), hi = cvt_e4m3x2(h.z * f, h.w * f);
+                        q[0] |= (lo & 0xffu) << (8 * i);
+                        q[1] |= (lo >> 8) << (8 * i);
+                        q[2] |= (hi & 0xffu) << (8 * i);
+                        q[3] |= (hi >> 8) << (8 * i);
+                    } else if (m < p.rows && n0 + c < p.N) {
+                        *reinterpret_cast<uint2*>(p.C + static_cast<size_t>(m) * p.N + n0 + c) = make_uint2(pack_bf16x2(h.x, h.y), pack_bf16x2(h.z, h.w));
+                    }
+                }
+                if constexpr (EPI == EPI_GATED_FP8)
+                    if (m0 + row < p.M)                             // M is a multiple of 16: both rows or none
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            *reinterpret_cast<uint16_t*>(p.epi.q_out + static_cast<size_t>(n0 + c + j) * p.M + m0 + row) = static_cast<uint16_t>(q[j]);
+            }
+        }
+        const int items = GATED ? 0 : (r1 - r0) * (BN / 4);
+        for (int idx = static_cast<int>(threadIdx.x) - 128; idx < items; idx += Cfg::PROMO_THREADS) {
+            const int row = r0 + idx / (BN / 4), c4 = idx % (BN / 4);
+            float4 sum = sum_at(row, c4 * 4);
+            const int m = m0 + row, n = n0 + c4 * 4;
+            if (m < p.rows && n < p.N) {
+                if constexpr (EPI == EPI_BIAS_ACT) sum = finish_4(sum, p.epi, m, n);
+                uint2 q;
+                q.x = pack_bf16x2(sum.x, sum.y);
+                q.y = pack_bf16x2(sum.z, sum.w);
+                *reinterpret_cast<uint2*>(p.C + static_cast<size_t>(m) * p.N + n) = q;
+            }
+        }
+    };
 
     if (warp < 4) {
         ptx::setmaxnreg_dec<64>();
@@ -772,6 +834,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
         }
         __syncwarp();
+        if constexpr (MODE == 2 && GATED) cluster_meet();
     } else {
         // -------------------------------------------------------- promotion + epilogue ------
         ptx::setmaxnreg_inc<216>();
@@ -805,7 +868,18 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     else
                         ptx::cp_async_16(dst + lane * 16, static_cast<const float*>(p.epi.bias) + (valid ? c : 0), valid);
                 }
-            const bool residual_here = EPI == EPI_BIAS_ACT && p.epi.residual && ncol0 < p.N && m0 + quarter * 32 < p.rows;
+            auto residual_here = [&]() { return p.epi.residual && ncol0 < p.N && m0 + quarter * 32 < p.rows; };
+            if constexpr (EPI == EPI_BIAS_ACT && MODE == 0)
+                if (residual_here() && ptx::elect_one()) {
+                    // The residual comes into the boxes the result leaves from, once the stores of the tile before have read them.  (Not
+                    // inside the K loop, after its first block: a test there cost 5 % of 6144 x 4608 x 7168.)
+                    ptx::tma_store_wait_read<0>();
+                    ptx::mbar_arrive_expect_tx(residual_bar(pw), 4096u * ((Cfg::NSTG == 2 && ncol1 < p.N) ? 2 : 1));
+                    ptx::tma_load_2d(my_stg_addr, &cmaps.m[MAP_RESIDUAL], ncol0, m0 + quarter * 32, residual_bar(pw));
+                    if (Cfg::NSTG == 2 && ncol1 < p.N)
+                        ptx::tma_load_2d(my_stg_addr + 4096, &cmaps.m[MAP_RESIDUAL], ncol1, m0 + quarter * 32, residual_bar(pw));
+                }
+            if constexpr (EPI == EPI_BIAS_ACT) __syncwarp();
             // running sums of this thread's row: 4 chunks of 32 columns, two fp32 per 64-bit register
             unsigned long long acc[Cfg::NCH][16];
 #pragma unroll
@@ -916,16 +990,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     ptx::fma32_from64<0>(acc[2 * q], v, s2);
                     ptx::fma32_from64<32>(acc[2 * q + 1], v, s2);
                 }
-                if constexpr (EPI == EPI_BIAS_ACT && MODE == 0) {
-                    // the residual comes into the boxes the result leaves from, once the stores of the tile before have read them
-                    if (kb == kb0 && residual_here && ptx::elect_one()) {
-                        ptx::tma_store_wait_read<0>();
-                        ptx::mbar_arrive_expect_tx(residual_bar(pw), 4096u * ((Cfg::NSTG == 2 && ncol1 < p.N) ? 2 : 1));
-                        ptx::tma_load_2d(my_stg_addr, &cmaps.m[MAP_RESIDUAL], ncol0, m0 + quarter * 32, residual_bar(pw));
-                        if (Cfg::NSTG == 2 && ncol1 < p.N)
-                            ptx::tma_load_2d(my_stg_addr + 4096, &cmaps.m[MAP_RESIDUAL], ncol1, m0 + quarter * 32, residual_bar(pw));
-                    }
-                }
                 if (pw == 0 && lane == 0) PROF_TRACE(5, ait);
                 if (pw == 1 && lane == 0) PROF_TRACE(8, ait);
                 PROF_ADD(t_fma);
@@ -976,7 +1040,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     for (int c = 0; c < Cfg::NCH; ++c)
                         bias_and_activate<decltype(act)::value>(acc[c], bias + c * 128, p.epi.bias != nullptr, p.epi);
                 });
-                if (residual_here) {
+                if (residual_here()) {
                     ok = wait_bounded(residual_bar(pw), tcount & 1u, abort_flag, p.status, DS_TIMEOUT_STAGE_FULL);
                     ok = __all_sync(0xffffffffu, ok);
                     ++tcount;                                           // residuals waited for
@@ -1005,9 +1069,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const unsigned long long g = acc[c][i], up = acc[c + 2][i];
-                            acc[c][i] = pack_f32x2(activate<decltype(act)::value>(f32x2_lo(g), p.epi) * f32x2_lo(up),
-                                                   activate<decltype(act)::value>(f32x2_hi(g), p.epi) * f32x2_hi(up));
+                            const unsigned long long g = activate_2<decltype(act)::value>(acc[c][i], p.epi), up = acc[c + 2][i];
+                            acc[c][i] = pack_f32x2(f32x2_lo(g) * f32x2_lo(up), f32x2_hi(g) * f32x2_hi(up));
                         }
                 });
                 // two boxes (or two 16 KB tiles of bytes), used in turn
@@ -1233,87 +1296,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         // C must have been read out of shared memory before the CTA goes away
         if (ptx::elect_one()) ptx::tma_store_wait_read<0>();
         __syncwarp();
+        if constexpr (MODE == 2 && GATED) {
+            cluster_meet();
+            cluster_reduce();
+        }
     }
 
-    if constexpr (MODE == 2) {
-        // ------------------------------------------------------------ cluster reduction ---
-        __syncthreads();                 // this CTA's partial tile is complete ...
-        ptx::cluster_sync();             // ... and so are those of the other K ranges of the tile
-        if (warp >= 4 && *abort_flag == 0u) {
-            const int S = p.splits;
-            const int my = static_cast<int>(ptx::cluster_ctarank());     // = this CTA's split index
-            int tile, m0, n0, kb0, kb1;
-            decode(static_cast<int>(blockIdx.x), tile, m0, n0, kb0, kb1);
-            // the rows this CTA finishes (gated fp8: pairs of rows)
-            const int r0 = EPI == EPI_GATED_FP8 ? 2 * ((64 * my) / S) : (128 * my) / S;
-            const int r1 = EPI == EPI_GATED_FP8 ? 2 * ((64 * (my + 1)) / S) : (128 * (my + 1)) / S;
-            uint32_t peer[8];
-#pragma unroll
-            for (int s = 0; s < 8; ++s) peer[s] = ptx::mapa(stage_base, static_cast<uint32_t>(s < S ? s : 0));
-            auto sum_at = [&](int row, int c) {                         // splits in fixed order: bit-deterministic
-                const uint32_t off = static_cast<uint32_t>(row * PART_PITCH + c * 4);
-                float4 v[8];
-#pragma unroll
-                for (int s = 0; s < 8; ++s)
-                    if (s < S) v[s] = ptx::ld_shared_cluster_v4(peer[s] + off);
-                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int s = 0; s < 8; ++s)
-                    if (s < S) { sum.x += v[s].x; sum.y += v[s].y; sum.z += v[s].z; sum.w += v[s].w; }
-                return sum;
-            };
-            if constexpr (GATED) {
-                // A warp takes a row (fp8: two neighbouring ones, a 16-bit store per column), a lane four columns.  Partial tiles are laid
-                // out [column group][first | second][64].
-                constexpr int ROWS = EPI == EPI_GATED_FP8 ? 2 : 1;
-                const int c = lane * 4, part = (c >> 6) * 128 + (c & 63);
-                for (int row = r0 + (warp - 4) * ROWS; row < r1; row += Cfg::PROMO_WARPS * ROWS) {
-                    uint32_t q[4] = {0u, 0u, 0u, 0u};
-#pragma unroll 1
-                    for (int i = 0; i < ROWS; ++i) {
-                        const float4 g = sum_at(row + i, part), up = sum_at(row + i, part + 64);
-                        float4 h;
-                        with_activation(p.epi, [&](auto act) {
-                            constexpr int A = decltype(act)::value;
-                            h = make_float4(activate<A>(g.x, p.epi) * up.x, activate<A>(g.y, p.epi) * up.y, activate<A>(g.z, p.epi) * up.z,
-                                            activate<A>(g.w, p.epi) * up.w);
-                        });
-                        const int m = m0 + row + i;
-                        if constexpr (EPI == EPI_GATED_FP8) {
-                            const float amax = warp_absmax_nan(max_nan(max_nan(fabsf(h.x), fabsf(h.y)), max_nan(fabsf(h.z), fabsf(h.w))));
-                            float inverse;
-                            const float f = scale_factor(amax, p.epi.fp8_max, inverse);
-                            if (lane == 0 && m < p.M) p.epi.scale_out[static_cast<size_t>(n0 >> 7) * p.M + m] = inverse;
-                            const uint32_t lo = cvt_e4m3x2(h.x * f, h.y * f), hi = cvt_e4m3x2(h.z * f, h.w * f);
-                            q[0] |= (lo & 0xffu) << (8 * i);
-                            q[1] |= (lo >> 8) << (8 * i);
-                            q[2] |= (hi & 0xffu) << (8 * i);
-                            q[3] |= (hi >> 8) << (8 * i);
-                        } else if (m < p.rows && n0 + c < p.N) {
-                            *reinterpret_cast<uint2*>(p.C + static_cast<size_t>(m) * p.N + n0 + c) = make_uint2(pack_bf16x2(h.x, h.y), pack_bf16x2(h.z, h.w));
-                        }
-                    }
-                    if constexpr (EPI == EPI_GATED_FP8)
-                        if (m0 + row < p.M)                             // M is a multiple of 16: both rows or none
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                *reinterpret_cast<uint16_t*>(p.epi.q_out + static_cast<size_t>(n0 + c + j) * p.M + m0 + row) = static_cast<uint16_t>(q[j]);
-                }
-            }
-            const int items = GATED ? 0 : (r1 - r0) * (BN / 4);
-            for (int idx = static_cast<int>(threadIdx.x) - 128; idx < items; idx += Cfg::PROMO_THREADS) {
-                const int row = r0 + idx / (BN / 4), c4 = idx % (BN / 4);
-                float4 sum = sum_at(row, c4 * 4);
-                const int m = m0 + row, n = n0 + c4 * 4;
-                if (m < p.rows && n < p.N) {
-                    if constexpr (EPI == EPI_BIAS_ACT) sum = finish_4(sum, p.epi, m, n);
-                    uint2 q;
-                    q.x = pack_bf16x2(sum.x, sum.y);
-                    q.y = pack_bf16x2(sum.z, sum.w);
-                    *reinterpret_cast<uint2*>(p.C + static_cast<size_t>(m) * p.N + n) = q;
-                }
-            }
-        }
+    if constexpr (MODE == 2 && !GATED) {
+        cluster_meet();
+        if (warp >= 4) cluster_reduce();
     }
 
     // ---------------------------------------------------------------- common exit -----

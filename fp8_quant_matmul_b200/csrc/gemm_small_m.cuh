@@ -305,10 +305,13 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                         for (int t = 0; t < 8; ++t)
                             r[t] = p.epi.residual && row0 + t0 + t < p.rows ? __bfloat162float(p.epi.residual[(row0 + t0 + t) * p.epi.ldr + n]) : 0.0f;
 #pragma unroll
-                        for (int t = 0; t < 8; ++t)
-                            if (row0 + t0 + t < p.rows)
-                                p.C[static_cast<size_t>(row0 + t0 + t) * p.N + n] =
-                                    __float2bfloat16_rn(activate<decltype(act)::value>(sum_of(0, t0 + t) + bias, p.epi) + r[t]);
+                        for (int t = 0; t < 8; t += 2) {
+                            const unsigned long long y =
+                                activate_2<decltype(act)::value>(ptx::add_f32x2(acc[(t0 + t) / 2], pack_f32x2(bias, bias)), p.epi);
+                            __nv_bfloat16* c = p.C + static_cast<size_t>(row0 + t0 + t) * p.N + n;
+                            if (row0 + t0 + t < p.rows) *c = __float2bfloat16_rn(f32x2_lo(y) + r[t]);
+                            if (row0 + t0 + t + 1 < p.rows) c[p.N] = __float2bfloat16_rn(f32x2_hi(y) + r[t + 1]);
+                        }
                     }
                 });
             } else {
@@ -361,12 +364,7 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                 };
                 float4 sum = sum_at(0);
                 if constexpr (GATED) {
-                    const float4 up = sum_at(1);
-                    with_activation(p.epi, [&](auto act) {
-                        constexpr int A = decltype(act)::value;
-                        sum = make_float4(activate<A>(sum.x, p.epi) * up.x, activate<A>(sum.y, p.epi) * up.y, activate<A>(sum.z, p.epi) * up.z,
-                                          activate<A>(sum.w, p.epi) * up.w);
-                    });
+                    sum = gate_4(sum, sum_at(1), p.epi);
                 }
                 if constexpr (EPI == EPI_GATED_FP8) {
                     // a warp's lanes are the 128 columns of row t

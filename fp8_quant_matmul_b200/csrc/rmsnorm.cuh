@@ -72,20 +72,9 @@ __device__ __forceinline__ float sum_16_rows(const float (&a)[16], int lane)
     return one + __shfl_xor_sync(0xffffffffu, one, 1);
 }
 
+using ptx::add_f32x2;
+using ptx::mul_f32x2;
 typedef unsigned long long f32x2;      // two fp32 values, the operand of the packed instructions
-
-__device__ __forceinline__ f32x2 mul_f32x2(f32x2 a, f32x2 b)
-{
-    f32x2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ f32x2 add_f32x2(f32x2 a, f32x2 b)
-{
-    f32x2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 
 // Four consecutive elements of a type, and as two pairs of fp32.
 template <class T>

@@ -139,7 +139,7 @@ def test_a_call_for_another_device_is_made_with_that_device_current(monkeypatch)
             seen.append((current[0], args))
             return 0
 
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
     monkeypatch.setattr(torch.cuda, "device", On)
     monkeypatch.setattr(api, "_stream", lambda index: 100 + index)
     monkeypatch.setattr(api, "lib", lambda: Lib())
