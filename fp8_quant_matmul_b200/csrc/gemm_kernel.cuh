@@ -311,21 +311,16 @@ __device__ __forceinline__ void stage_and_store_2x64(const CUtensorMap* tmC, int
     }
 }
 
-// v = act(v + bias): bias from shared memory (64 fp32), or none.
-template <int ACT>
-__device__ __forceinline__ void bias_and_activate(unsigned long long (&v)[16], uint32_t bias_addr, bool has_bias, const Epilogue& e)
+// v = v + bias of 32 columns, fp32 in shared memory.
+__device__ __forceinline__ void add_bias(unsigned long long (&v)[16], uint32_t bias_addr)
 {
-    if (has_bias)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            unsigned long long b0, b1;
-            ptx::ld_shared_v2_b64(bias_addr + static_cast<uint32_t>(16 * i), b0, b1);
-            v[2 * i] = pack_f32x2(f32x2_lo(v[2 * i]) + f32x2_lo(b0), f32x2_hi(v[2 * i]) + f32x2_hi(b0));
-            v[2 * i + 1] = pack_f32x2(f32x2_lo(v[2 * i + 1]) + f32x2_lo(b1), f32x2_hi(v[2 * i + 1]) + f32x2_hi(b1));
-        }
-    if constexpr (ACT != ACT_NONE)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = activate_2<ACT>(v[i], e);
+    for (int i = 0; i < 8; ++i) {
+        unsigned long long b0, b1;
+        ptx::ld_shared_v2_b64(bias_addr + static_cast<uint32_t>(16 * i), b0, b1);
+        v[2 * i] = pack_f32x2(f32x2_lo(v[2 * i]) + f32x2_lo(b0), f32x2_hi(v[2 * i]) + f32x2_hi(b0));
+        v[2 * i + 1] = pack_f32x2(f32x2_lo(v[2 * i + 1]) + f32x2_lo(b1), f32x2_hi(v[2 * i + 1]) + f32x2_hi(b1));
+    }
 }
 // stage_64 onto the residual that lies in the box.
 __device__ __forceinline__ void add_and_stage_64(uint8_t* stg, int lane, const unsigned long long (&c0)[16], const unsigned long long (&c1)[16])
@@ -1034,11 +1029,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                         reinterpret_cast<uint4*>(raw)[lane] = make_uint4(w.x << 16, w.x & 0xffff0000u, w.y << 16, w.y & 0xffff0000u);
                     }
                     __syncwarp();
+#pragma unroll
+                    for (int c = 0; c < Cfg::NCH; ++c) add_bias(acc[c], bias + c * 128);
                 }
                 with_activation(p.epi, [&](auto act) {
+                    if constexpr (decltype(act)::value != ACT_NONE)
 #pragma unroll
-                    for (int c = 0; c < Cfg::NCH; ++c)
-                        bias_and_activate<decltype(act)::value>(acc[c], bias + c * 128, p.epi.bias != nullptr, p.epi);
+                        for (int c = 0; c < Cfg::NCH; ++c)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) acc[c][i] = activate_2<decltype(act)::value>(acc[c][i], p.epi);
                 });
                 if (residual_here()) {
                     ok = wait_bounded(residual_bar(pw), tcount & 1u, abort_flag, p.status, DS_TIMEOUT_STAGE_FULL);
