@@ -476,9 +476,11 @@ static Config plan(const DeviceModel& dm, int device, int M, int N, int K, int p
 }
 
 // The configuration of a fused call (gated: two products, N columns of each).  Those of the estimate that are built for it: the full-K
-// kernel on 128-wide (gated: 2 x 128-wide) and pair tiles, the cluster reduction, few rows.  They need no workspace, and what the
-// epilogue adds to a tile hardly differs between them.
-static int choose_fused(const DeviceModel& dm, int M, int N, int K, bool gated, int splits, int tile_n, Config* out)
+// kernel on 128-wide (gated: 2 x 128-wide) and pair tiles, the cluster reduction, few rows.  They need no workspace.
+// An activation takes longer on the wide tiles, whose promotion threads own 128 columns instead of 64 and whose MMAs are only two K blocks
+// ahead: 2.2 us per wave (0.3 on 128-wide tiles).  silu and bias, pair / 128-wide: 2960 x 1920 x 640 15.4 / 12.5 us, 6720 x 1488 x 512 20.2 / 17.4,
+// 4096 x 7168 x 512 38.3 / 35.1, 6144 x 4608 x 1024 42.4 / 44.7, 1440 x 1664 x 2304 14.6 / 15.6.  Gated, all are wide.
+static int choose_fused(const DeviceModel& dm, int M, int N, int K, bool gated, bool activation, int splits, int tile_n, Config* out)
 {
     const int KB = K / 128, t = tile_n & ~FP8BS_SMALL_M;
     if (splits < 0 || splits > MAX_CLUSTER_SPLITS || splits > KB) return FP8BS_ERR_ARG;
@@ -495,9 +497,11 @@ static int choose_fused(const DeviceModel& dm, int M, int N, int K, bool gated, 
             if (t && t != (tn | (cg == 2 ? FP8BS_TILE_PAIR : 0))) continue;
             for (int s = 1; s <= MAX_CLUSTER_SPLITS && s <= KB; ++s) {
                 if (splits && s != splits) continue;
-                if (s > 1 && (cg == 2 || dm.max_clusters[s] < 1)) continue;
+                if (s > 1 ? (cg == 2 || dm.max_clusters[s] < 1) : dm.sm_count < cg) continue;
                 if (s == 1 && cg == 1 && !gated && tn == 256) continue;            // not built
-                const double c = config_cost(dm, M, gated ? 256 * ceil_div(N, 128) : N, K, tn, s, cg, s > 1 ? 2 : 0);
+                double c = config_cost(dm, M, gated ? 256 * ceil_div(N, 128) : N, K, tn, s, cg, s > 1 ? 2 : 0);
+                if (!gated && activation && s == 1)
+                    c += (cg == 2 ? 2.2 : 0.3) * ceil_div(ceil_div(M, 128 * cg) * ceil_div(N, tn), dm.sm_count / cg);
                 if (c < best_cost) {
                     best_cost = c;
                     *out = Config{s > 1 ? FP8BS_PATH_MN_SMALL : FP8BS_PATH_MN_LARGE, tn, s, cg, s > 1 ? 2 : 0, 0};
@@ -911,7 +915,9 @@ static int fused_impl(const void* A, const void* B, const void* B2, const float*
     DeviceInfo* dev = nullptr;
     const int dev_rc = device_setup(&dev);
     Config cfg{};
-    if ((rc = choose_fused(dev_rc == FP8BS_OK ? dev->model : kB200Model, M, N, K, gated, splits, tile_n, &cfg))) return rc;
+    if ((rc = choose_fused(dev_rc == FP8BS_OK ? dev->model : kB200Model, M, N, K, gated, activation != FP8BS_ACT_NONE, splits, tile_n,
+                           &cfg)))
+        return rc;
     if (dev_rc) return dev_rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     TensorMaps tm{};
