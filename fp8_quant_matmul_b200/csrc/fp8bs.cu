@@ -668,7 +668,7 @@ static int launch_clusters(Kernel kernel, int ctas, int cluster, int threads, in
 }
 
 template <int BN, int CG, int MODE, int EPI = EPI_NONE>
-static int launch(const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t stream)
+static int launch(const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t stream, const EpiArg<EPI>& e = {})
 {
     using Cfg = TileCfg<BN, CG>;
     const int units = p.m_tiles * p.n_tiles * p.splits;
@@ -676,35 +676,41 @@ static int launch(const TensorMaps& tm, const GemmParams& p, int sm_count, cudaS
     if (MODE == 2) groups = units;                                  // one CTA per (tile, K range); a cluster per tile
     if (MODE == 3) groups = stream_k_ctas(p.m_tiles * p.n_tiles, p.K / 128, sm_count);
     return launch_clusters(gemm_kernel<BN, CG, MODE, EPI>, groups * CG, MODE == 2 ? p.splits : CG, Cfg::THREADS,
-                           Cfg::SMEM_BYTES + epi_smem(EPI), stream, tm.A, tm.B, tm.C, p);
+                           Cfg::SMEM_BYTES + epi_smem(EPI), stream, tm.A, tm.B, tm.C, p, e);
 }
 
 template <int T, int EPI = EPI_NONE>
-static int launch_small_m(const TensorMaps& tm, const GemmParams& p, cudaStream_t stream)
+static int launch_small_m(const TensorMaps& tm, const GemmParams& p, cudaStream_t stream, const EpiArg<EPI>& e = {})
 {
     using Cfg = SmallMCfg<T, EPI>;
-    return launch_clusters(gemm_small_m_kernel<T, EPI>, p.n_tiles * p.splits, p.splits, Cfg::THREADS, Cfg::SMEM_BYTES, stream, tm.A, tm.B,
-                           tm.C.m[MAP_UP], p);
+    SecondMap<EPI> up{};
+    if constexpr (Cfg::GATED) up = tm.C.m[MAP_UP];
+    return launch_clusters(gemm_small_m_kernel<T, EPI>, p.n_tiles * p.splits, p.splits, Cfg::THREADS, Cfg::SMEM_BYTES, stream, tm.A, tm.B, p, up, e);
+}
+
+template <int EPI>
+static int launch_fused_small_m(const TensorMaps& tm, const GemmParams& p, cudaStream_t st, const EpiArg<EPI>& e)
+{
+    return p.M <= 16 ? launch_small_m<16, EPI>(tm, p, st, e) : p.M <= 32 ? launch_small_m<32, EPI>(tm, p, st, e) : launch_small_m<64, EPI>(tm, p, st, e);
 }
 
 // The fused calls: bias, activation and residual on 128-wide and pair tiles, or in the cluster reduction ...
-static int launch_bias_act(const Config& c, const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t st)
+static int launch_bias_act(const Config& c, const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t st, const Epilogue& epilogue)
 {
-    if (c.mode == 5)
-        return p.M <= 16 ? launch_small_m<16, EPI_BIAS_ACT>(tm, p, st) : p.M <= 32 ? launch_small_m<32, EPI_BIAS_ACT>(tm, p, st)
-                                                                       : launch_small_m<64, EPI_BIAS_ACT>(tm, p, st);
-    if (c.mode == 2)
-        return c.tile_n == 256 ? launch<256, 1, 2, EPI_BIAS_ACT>(tm, p, sm_count, st) : launch<128, 1, 2, EPI_BIAS_ACT>(tm, p, sm_count, st);
-    return c.cg == 2 ? launch<256, 2, 0, EPI_BIAS_ACT>(tm, p, sm_count, st) : launch<128, 1, 0, EPI_BIAS_ACT>(tm, p, sm_count, st);
+    constexpr int EPI = EPI_BIAS_ACT;
+    const EpiArg<EPI> e{epilogue};
+    if (c.mode == 5) return launch_fused_small_m<EPI>(tm, p, st, e);
+    if (c.mode == 2) return c.tile_n == 256 ? launch<256, 1, 2, EPI>(tm, p, sm_count, st, e) : launch<128, 1, 2, EPI>(tm, p, sm_count, st, e);
+    return c.cg == 2 ? launch<256, 2, 0, EPI>(tm, p, sm_count, st, e) : launch<128, 1, 0, EPI>(tm, p, sm_count, st, e);
 }
 // ... and the gated pair of products, on tiles of 2 x 128 columns.
 template <int EPI>
-static int launch_gated(const Config& c, const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t st)
+static int launch_gated(const Config& c, const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t st, const Epilogue& epilogue)
 {
-    if (c.mode == 5)
-        return p.M <= 16 ? launch_small_m<16, EPI>(tm, p, st) : p.M <= 32 ? launch_small_m<32, EPI>(tm, p, st) : launch_small_m<64, EPI>(tm, p, st);
-    if (c.mode == 2) return launch<256, 1, 2, EPI>(tm, p, sm_count, st);
-    return c.cg == 2 ? launch<256, 2, 0, EPI>(tm, p, sm_count, st) : launch<256, 1, 0, EPI>(tm, p, sm_count, st);
+    const EpiArg<EPI> e{epilogue};
+    if (c.mode == 5) return launch_fused_small_m<EPI>(tm, p, st, e);
+    if (c.mode == 2) return launch<256, 1, 2, EPI>(tm, p, sm_count, st, e);
+    return c.cg == 2 ? launch<256, 2, 0, EPI>(tm, p, sm_count, st, e) : launch<256, 1, 0, EPI>(tm, p, sm_count, st, e);
 }
 
 // How many clusters of `cluster` CTAs with `warps` warps of the norm kernel run at once: asked once per device, type and shape.
@@ -928,7 +934,7 @@ static int fused_impl(const void* A, const void* B, const void* B2, const float*
     if (residual && cfg.mode == 0 && (rc = encode_c_map(&tm.C.m[MAP_RESIDUAL], const_cast<void*>(residual), rows, N, ldr))) return rc;
     GemmParams p = gemm_params(cfg, gated ? 128 : cfg.tile_n, a_scale, b_scale, out, M, N, K, 0, N, dev->status_ptr, st);
     p.rows = rows;
-    Epilogue& e = p.epi;
+    Epilogue e{};
     e.bias = bias;
     e.residual = static_cast<const __nv_bfloat16*>(residual);
     e.ldr = ldr;
@@ -946,8 +952,8 @@ static int fused_impl(const void* A, const void* B, const void* B2, const float*
             e.lowest = -7.4f; break;
         default: e.act = ACT_NONE;
     }
-    if (!gated) return launch_bias_act(cfg, tm, p, dev->sm_count, st);
-    return fp8 ? launch_gated<EPI_GATED_FP8>(cfg, tm, p, dev->sm_count, st) : launch_gated<EPI_GATED>(cfg, tm, p, dev->sm_count, st);
+    if (!gated) return launch_bias_act(cfg, tm, p, dev->sm_count, st, e);
+    return fp8 ? launch_gated<EPI_GATED_FP8>(cfg, tm, p, dev->sm_count, st, e) : launch_gated<EPI_GATED>(cfg, tm, p, dev->sm_count, st, e);
 }
 
 // ---------------------------------------------------------------------------------------

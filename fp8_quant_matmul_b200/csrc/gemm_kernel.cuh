@@ -112,7 +112,6 @@ struct GemmParams {
     int n_dest;              // number of valid entries of the CMaps argument (1 = only the caller's C)
     int rows;                // rows of C that exist: M, fewer in the fused calls
     float elem_scale;        // folded into b_scale: 1 for e4m3fn bytes
-    Epilogue epi;            // EPI != 0 only
 #ifdef FP8BS_PROFILE
     long long* prof;         // per CTA: 8 cycle counters (profiling builds only)
 #endif
@@ -130,6 +129,15 @@ constexpr int EPI_BIAS_BYTES = 8 * 512;              // per promotion warp: the 
 constexpr int epi_smem(int epi) { return epi == EPI_NONE ? 0 : EPI_BIAS_BYTES; }
 // CMaps entries of the fused calls behind C (entry 0; gated fp8: the bytes of h)
 constexpr int MAP_RESIDUAL = 1, MAP_UP = 1;
+// The kernels' last parameter: nothing where there is no fused epilogue (a longer list of parameters is paid at every launch).
+template <int EPI>
+struct EpiArg {
+    Epilogue e;
+};
+template <>
+struct EpiArg<EPI_NONE> {
+    static constexpr Epilogue e = {};
+};
 
 template <int BN, int CG>
 struct TileCfg {
@@ -373,7 +381,7 @@ __global__ void wait_timeout_selftest_kernel(unsigned int* status, long long lim
 template <int BN, int CG, int MODE, int EPI = EPI_NONE>
 __global__ void __launch_bounds__(TileCfg<BN, CG>::THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-            const __grid_constant__ CMaps cmaps, const GemmParams p)
+            const __grid_constant__ CMaps cmaps, const GemmParams p, const EpiArg<EPI> ea)
 {
     using Cfg = TileCfg<BN, CG>;
     constexpr int STAGES = Cfg::STAGES;
@@ -426,7 +434,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         ptx::prefetch_tensormap(&tmA);
         ptx::prefetch_tensormap(&tmB);
         for (int d = 0; d < p.n_dest; ++d) ptx::prefetch_tensormap(&cmaps.m[d]);
-        if (GATED || (EPI == EPI_BIAS_ACT && MODE == 0 && p.epi.residual)) ptx::prefetch_tensormap(&cmaps.m[1]);
+        if (GATED || (EPI == EPI_BIAS_ACT && MODE == 0 && ea.e.residual)) ptx::prefetch_tensormap(&cmaps.m[1]);
         for (int s = 0; s < STAGES; ++s) {
             ptx::mbar_init(full_bar(s), 1);
             ptx::mbar_init(empty_bar(s), 1);
@@ -560,13 +568,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll 1
             for (int row = r0 + warp - 4; row < r1; row += Cfg::PROMO_WARPS) {
                 const float4 g = sum_at(row, part), up = sum_at(row, part + 64);
-                const float4 h = gate_4(g, up, p.epi);
+                const float4 h = gate_4(g, up, ea.e);
                 const int m = m0 + row;
                 if constexpr (EPI == EPI_GATED_FP8) {
                     const float amax = warp_absmax_nan(max_nan(max_nan(fabsf(h.x), fabsf(h.y)), max_nan(fabsf(h.z), fabsf(h.w))));
                     float inverse;
-                    const float f = scale_factor(amax, p.epi.fp8_max, inverse);
-                    if (lane == 0 && m < p.M) p.epi.scale_out[static_cast<size_t>(n0 >> 7) * p.M + m] = inverse;
+                    const float f = scale_factor(amax, ea.e.fp8_max, inverse);
+                    if (lane == 0 && m < p.M) ea.e.scale_out[static_cast<size_t>(n0 >> 7) * p.M + m] = inverse;
                     const uint32_t lo = cvt_e4m3x2(h.x * f, h.y * f), hi = cvt_e4m3x2(h.z * f, h.w * f);
                     uint8_t* at = stg_ptr + c * PITCH + (row - r0);
                     at[0] = static_cast<uint8_t>(lo);
@@ -583,7 +591,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     const int k = idx & 127, r = (idx >> 7) * 16;
                     const uint32_t* from = reinterpret_cast<const uint32_t*>(stg_ptr + k * PITCH + r);
                     if (m0 + r0 + r < p.M)                   // M is a multiple of 16: all 16 rows or none
-                        *reinterpret_cast<uint4*>(p.epi.q_out + static_cast<size_t>(n0 + k) * p.M + m0 + r0 + r) =
+                        *reinterpret_cast<uint4*>(ea.e.q_out + static_cast<size_t>(n0 + k) * p.M + m0 + r0 + r) =
                             make_uint4(from[0], from[1], from[2], from[3]);
                 }
             }
@@ -594,7 +602,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             float4 sum = sum_at(row, c4 * 4);
             const int m = m0 + row, n = n0 + c4 * 4;
             if (m < p.rows && n < p.N) {
-                if constexpr (EPI == EPI_BIAS_ACT) sum = finish_4(sum, p.epi, m, n);
+                if constexpr (EPI == EPI_BIAS_ACT) sum = finish_4(sum, ea.e, m, n);
                 uint2 q;
                 q.x = pack_bf16x2(sum.x, sum.y);
                 q.y = pack_bf16x2(sum.z, sum.w);
@@ -781,7 +789,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 const float* ap = p.a_scale + static_cast<size_t>(fkb) * p.M + fm;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) a[j] = (fm + 32 * j < p.M) ? __ldg(ap + 32 * j) : 0.0f;
-                b = __ldg((GATED && (lane & 1) ? p.epi.up_scale : p.b_scale) + static_cast<size_t>(fkb) * p.sn + fnb);
+                const float* bp = p.b_scale;
+                if constexpr (GATED) bp = (lane & 1) ? ea.e.up_scale : bp;
+                b = __ldg(bp + static_cast<size_t>(fkb) * p.sn + fnb);
                 if (++fkb == fkb1) {
                     fu += unit_step;
                     fetch_unit();
@@ -858,17 +868,17 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             const int ncol0 = GATED ? n0 + grp * 64 : n0 + col_of(grp, 0);      // first local columns of this thread's pieces
             const int ncol1 = n0 + col_of(grp, 1);
             if constexpr (EPI == EPI_BIAS_ACT && MODE == 0)
-                if (p.epi.bias) {
+                if (ea.e.bias) {
                     // the bias of this warp's columns, four per lane; the last tile's has been used (its staging ended in a __syncwarp)
                     const int c = (lane < 16 ? ncol0 : ncol1) + (lane & 15) * 4;
                     const bool valid = c < p.N && lane < 16 * Cfg::QUADS;
                     const uint32_t dst = epi_base + static_cast<uint32_t>(pw * 512);
-                    if (p.epi.bias_is_bf16)
-                        ptx::cp_async_8(dst + lane * 8, static_cast<const __nv_bfloat16*>(p.epi.bias) + (valid ? c : 0), valid);
+                    if (ea.e.bias_is_bf16)
+                        ptx::cp_async_8(dst + lane * 8, static_cast<const __nv_bfloat16*>(ea.e.bias) + (valid ? c : 0), valid);
                     else
-                        ptx::cp_async_16(dst + lane * 16, static_cast<const float*>(p.epi.bias) + (valid ? c : 0), valid);
+                        ptx::cp_async_16(dst + lane * 16, static_cast<const float*>(ea.e.bias) + (valid ? c : 0), valid);
                 }
-            auto residual_here = [&]() { return p.epi.residual && ncol0 < p.N && m0 + quarter * 32 < p.rows; };
+            auto residual_here = [&]() { return ea.e.residual && ncol0 < p.N && m0 + quarter * 32 < p.rows; };
             if constexpr (EPI == EPI_BIAS_ACT && MODE == 0)
                 if (residual_here() && ptx::elect_one()) {
                     // The residual comes into the boxes the result leaves from, once the stores of the tile before have read them.  (Not
@@ -1024,9 +1034,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             if constexpr (MODE == 0 && EPI == EPI_BIAS_ACT) {
                 if (!ok) break;
                 const uint32_t bias = epi_base + static_cast<uint32_t>(pw * 512);
-                if (p.epi.bias) {
+                if (ea.e.bias) {
                     ptx::cp_async_wait_all();
-                    if (p.epi.bias_is_bf16) {
+                    if (ea.e.bias_is_bf16) {
                         // widened in place: a lane's own four, after every lane has read its own
                         uint2* raw = reinterpret_cast<uint2*>(stg_ptr + (bias - stg_base));
                         const uint2 w = raw[lane];
@@ -1037,12 +1047,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
                     for (int c = 0; c < Cfg::NCH; ++c) add_bias(acc[c], bias + c * 128);
                 }
-                with_activation(p.epi, [&](auto act) {
+                with_activation(ea.e, [&](auto act) {
                     if constexpr (decltype(act)::value != ACT_NONE)
 #pragma unroll
                         for (int c = 0; c < Cfg::NCH; ++c)
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) acc[c][i] = activate_2<decltype(act)::value>(acc[c][i], p.epi);
+                            for (int i = 0; i < 16; ++i) acc[c][i] = activate_2<decltype(act)::value>(acc[c][i], ea.e);
                 });
                 if (residual_here()) {
                     ok = wait_bounded(residual_bar(pw), tcount & 1u, abort_flag, p.status, DS_TIMEOUT_STAGE_FULL);
@@ -1068,12 +1078,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             } else if constexpr (MODE == 0 && GATED) {
                 if (EPI == EPI_GATED && !ok) break;
                 // h = act(first) * second, in the registers of the first
-                with_activation(p.epi, [&](auto act) {
+                with_activation(ea.e, [&](auto act) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const unsigned long long g = activate_2<decltype(act)::value>(acc[c][i], p.epi), up = acc[c + 2][i];
+                            const unsigned long long g = activate_2<decltype(act)::value>(acc[c][i], ea.e), up = acc[c + 2][i];
                             acc[c][i] = pack_f32x2(f32x2_lo(g) * f32x2_lo(up), f32x2_hi(g) * f32x2_hi(up));
                         }
                 });
@@ -1102,9 +1112,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     if (pw == 0 && ptx::elect_one()) ptx::tma_store_wait_read<1>();
                     if (promo_any<Cfg::PROMO_THREADS>(!ok)) { ok = false; break; }
                     float inverse;
-                    const float f = scale_factor(max_nan(mine, row_max[(grp ^ 1) * 128]), p.epi.fp8_max, inverse);
+                    const float f = scale_factor(max_nan(mine, row_max[(grp ^ 1) * 128]), ea.e.fp8_max, inverse);
                     if (grp == 0 && m0 + row_in_tile < p.M && n0 < p.N)
-                        p.epi.scale_out[static_cast<size_t>(n0 >> 7) * p.M + m0 + row_in_tile] = inverse;
+                        ea.e.scale_out[static_cast<size_t>(n0 >> 7) * p.M + m0 + row_in_tile] = inverse;
                     // byte (k, row) of the tile, as a 128-byte-swizzled store box {128 rows, 128 k} expects it
                     uint8_t* bytes = stg_ptr + turn * 16384 + grp * 64 * 128 + (row_in_tile & 15);
 #pragma unroll

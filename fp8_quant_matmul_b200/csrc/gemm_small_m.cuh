@@ -76,11 +76,15 @@ __device__ __forceinline__ void tmem_ld_x32_sync(uint32_t taddr, uint32_t (&v)[3
 }
 
 // grid = n_tiles * splits CTAs, cluster size = splits.
-// tmU: the second matrix (gated; otherwise not used).
+// The second matrix of the gated form; no parameter otherwise.
+struct NoMap {};
+template <int EPI>
+using SecondMap = typename std::conditional<EPI == EPI_GATED || EPI == EPI_GATED_FP8, CUtensorMap, NoMap>::type;
+
 template <int T, int EPI = EPI_NONE>
 __global__ void __launch_bounds__((SmallMCfg<T, EPI>::THREADS), (SmallMCfg<T, EPI>::CTAS))
-gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmU,
-                    const GemmParams p)
+gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const GemmParams p,
+                    const __grid_constant__ SecondMap<EPI> tmU, const EpiArg<EPI> ea)
 {
     using Cfg = SmallMCfg<T, EPI>;
     constexpr bool GATED = Cfg::GATED;
@@ -223,7 +227,11 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    b[h] = __ldg((GATED && h ? p.epi.up_scale : p.b_scale) + static_cast<size_t>(fkb) * p.sn + nb[GATED ? 0 : h]) * p.elem_scale;
+                    {
+                        const float* bp = p.b_scale;
+                        if constexpr (GATED) bp = h ? ea.e.up_scale : bp;
+                        b[h] = __ldg(bp + static_cast<size_t>(fkb) * p.sn + nb[GATED ? 0 : h]) * p.elem_scale;
+                    }
             }
             ++fkb;
         };
@@ -296,18 +304,18 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
         const int n = n0 + (warp & 3) * 32 + lane;
         if (warp < Cfg::PROMO_WARPS && ok && n < p.N) {
             if constexpr (EPI == EPI_BIAS_ACT) {
-                const float bias = p.epi.bias ? bias_1(p.epi, n) : 0.0f;
-                with_activation(p.epi, [&](auto act) {
+                const float bias = ea.e.bias ? bias_1(ea.e, n) : 0.0f;
+                with_activation(ea.e, [&](auto act) {
 #pragma unroll
                     for (int t0 = 0; t0 < TW; t0 += 8) {               // eight residuals in flight
                         float r[8];
 #pragma unroll
                         for (int t = 0; t < 8; ++t)
-                            r[t] = p.epi.residual && row0 + t0 + t < p.rows ? __bfloat162float(p.epi.residual[(row0 + t0 + t) * p.epi.ldr + n]) : 0.0f;
+                            r[t] = ea.e.residual && row0 + t0 + t < p.rows ? __bfloat162float(ea.e.residual[(row0 + t0 + t) * ea.e.ldr + n]) : 0.0f;
 #pragma unroll
                         for (int t = 0; t < 8; t += 2) {
                             const unsigned long long y =
-                                activate_2<decltype(act)::value>(ptx::add_f32x2(acc[(t0 + t) / 2], pack_f32x2(bias, bias)), p.epi);
+                                activate_2<decltype(act)::value>(ptx::add_f32x2(acc[(t0 + t) / 2], pack_f32x2(bias, bias)), ea.e);
                             __nv_bfloat16* c = p.C + static_cast<size_t>(row0 + t0 + t) * p.N + n;
                             if (row0 + t0 + t < p.rows) *c = __float2bfloat16_rn(f32x2_lo(y) + r[t]);
                             if (row0 + t0 + t + 1 < p.rows) c[p.N] = __float2bfloat16_rn(f32x2_hi(y) + r[t + 1]);
@@ -364,22 +372,22 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                 };
                 float4 sum = sum_at(0);
                 if constexpr (GATED) {
-                    sum = gate_4(sum, sum_at(1), p.epi);
+                    sum = gate_4(sum, sum_at(1), ea.e);
                 }
                 if constexpr (EPI == EPI_GATED_FP8) {
                     // a warp's lanes are the 128 columns of row t
                     const float amax = warp_absmax_nan(max_nan(max_nan(fabsf(sum.x), fabsf(sum.y)), max_nan(fabsf(sum.z), fabsf(sum.w))));
                     float inverse;
-                    const float f = scale_factor(amax, p.epi.fp8_max, inverse);
-                    if ((idx & 31) == 0) p.epi.scale_out[static_cast<size_t>(n0 >> 7) * p.M + t0 + t] = inverse;
+                    const float f = scale_factor(amax, ea.e.fp8_max, inverse);
+                    if ((idx & 31) == 0) ea.e.scale_out[static_cast<size_t>(n0 >> 7) * p.M + t0 + t] = inverse;
                     const uint32_t lo = cvt_e4m3x2(sum.x * f, sum.y * f), hi = cvt_e4m3x2(sum.z * f, sum.w * f);
-                    uint8_t* dst = p.epi.q_out + static_cast<size_t>(n0 + c) * p.M + t0 + t;
+                    uint8_t* dst = ea.e.q_out + static_cast<size_t>(n0 + c) * p.M + t0 + t;
                     dst[0] = static_cast<uint8_t>(lo);
                     dst[p.M] = static_cast<uint8_t>(lo >> 8);
                     dst[2 * p.M] = static_cast<uint8_t>(hi);
                     dst[3 * p.M] = static_cast<uint8_t>(hi >> 8);
                 } else if (n0 + c < p.N && t0 + t < p.rows) {
-                    if constexpr (EPI == EPI_BIAS_ACT) sum = finish_4(sum, p.epi, t0 + t, n0 + c);
+                    if constexpr (EPI == EPI_BIAS_ACT) sum = finish_4(sum, ea.e, t0 + t, n0 + c);
                     uint2 q;
                     q.x = pack_bf16x2(sum.x, sum.y);
                     q.y = pack_bf16x2(sum.z, sum.w);
