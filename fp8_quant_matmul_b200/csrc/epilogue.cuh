@@ -113,11 +113,11 @@ __device__ __forceinline__ unsigned long long activate_2(unsigned long long x, c
 }
 // f(integral constant of the activation): one branch per call of this, not per element.
 template <class F>
-__device__ __forceinline__ void with_activation(const Epilogue& e, F f)
+__device__ __forceinline__ void with_activation(int which, F f)
 {
-    if (e.act == ACT_LOGISTIC) f(std::integral_constant<int, ACT_LOGISTIC>{});
-    else if (e.act == ACT_ERF) f(std::integral_constant<int, ACT_ERF>{});
-    else if (e.act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
+    if (which == ACT_LOGISTIC) f(std::integral_constant<int, ACT_LOGISTIC>{});
+    else if (which == ACT_ERF) f(std::integral_constant<int, ACT_ERF>{});
+    else if (which == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
     else f(std::integral_constant<int, ACT_NONE>{});
 }
 
@@ -139,7 +139,7 @@ __device__ __forceinline__ float bias_1(const Epilogue& e, int n)
 __device__ __forceinline__ float4 activate_4(float4 v, const Epilogue& e)
 {
     unsigned long long a = pack_f32x2(v.x, v.y), b = pack_f32x2(v.z, v.w);
-    with_activation(e, [&](auto act) {
+    with_activation(e.act, [&](auto act) {
         a = activate_2<decltype(act)::value>(a, e);
         b = activate_2<decltype(act)::value>(b, e);
     });

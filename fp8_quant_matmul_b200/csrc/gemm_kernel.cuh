@@ -862,23 +862,31 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         uint32_t tcount = 0;                     // MODE 4: tiles done by this CTA
         bool ok = true;
         PROF_DECL(w_tfull); PROF_DECL(t_fma); PROF_DECL(t_epi);
+        // What a tile has to know of its epilogue, in a register that the compiler takes as given: read from the parameters anew for every
+        // tile it came from beyond the constant cache.
+        int epi_flags = 0;
+        constexpr int HAS_BIAS = 4, BIAS_BF16 = 8, HAS_RESIDUAL = 16, ACT_MASK = 3;
+        if constexpr (EPI != EPI_NONE) {
+            epi_flags = ea.e.act | (ea.e.bias ? HAS_BIAS : 0) | (ea.e.bias_is_bf16 ? BIAS_BF16 : 0) | (ea.e.residual ? HAS_RESIDUAL : 0);
+            asm volatile("" : "+r"(epi_flags));
+        }
         for (int u = unit0; u < units; u += unit_step) {
             int tile, m0, n0, kb0, kb1;
             decode(u, tile, m0, n0, kb0, kb1);
             const int ncol0 = GATED ? n0 + grp * 64 : n0 + col_of(grp, 0);      // first local columns of this thread's pieces
             const int ncol1 = n0 + col_of(grp, 1);
             if constexpr (EPI == EPI_BIAS_ACT && MODE == 0)
-                if (ea.e.bias) {
+                if (epi_flags & HAS_BIAS) {
                     // the bias of this warp's columns, four per lane; the last tile's has been used (its staging ended in a __syncwarp)
                     const int c = (lane < 16 ? ncol0 : ncol1) + (lane & 15) * 4;
                     const bool valid = c < p.N && lane < 16 * Cfg::QUADS;
                     const uint32_t dst = epi_base + static_cast<uint32_t>(pw * 512);
-                    if (ea.e.bias_is_bf16)
+                    if (epi_flags & BIAS_BF16)
                         ptx::cp_async_8(dst + lane * 8, static_cast<const __nv_bfloat16*>(ea.e.bias) + (valid ? c : 0), valid);
                     else
                         ptx::cp_async_16(dst + lane * 16, static_cast<const float*>(ea.e.bias) + (valid ? c : 0), valid);
                 }
-            auto residual_here = [&]() { return ea.e.residual && ncol0 < p.N && m0 + quarter * 32 < p.rows; };
+            auto residual_here = [&]() { return (epi_flags & HAS_RESIDUAL) && ncol0 < p.N && m0 + quarter * 32 < p.rows; };
             if constexpr (EPI == EPI_BIAS_ACT && MODE == 0)
                 if (residual_here() && ptx::elect_one()) {
                     // The residual comes into the boxes the result leaves from, once the stores of the tile before have read them.  (Not
@@ -1034,9 +1042,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             if constexpr (MODE == 0 && EPI == EPI_BIAS_ACT) {
                 if (!ok) break;
                 const uint32_t bias = epi_base + static_cast<uint32_t>(pw * 512);
-                if (ea.e.bias) {
+                if (epi_flags & HAS_BIAS) {
                     ptx::cp_async_wait_all();
-                    if (ea.e.bias_is_bf16) {
+                    if (epi_flags & BIAS_BF16) {
                         // widened in place: a lane's own four, after every lane has read its own
                         uint2* raw = reinterpret_cast<uint2*>(stg_ptr + (bias - stg_base));
                         const uint2 w = raw[lane];
@@ -1047,7 +1055,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
                     for (int c = 0; c < Cfg::NCH; ++c) add_bias(acc[c], bias + c * 128);
                 }
-                with_activation(ea.e, [&](auto act) {
+                with_activation(epi_flags & ACT_MASK, [&](auto act) {
                     if constexpr (decltype(act)::value != ACT_NONE)
 #pragma unroll
                         for (int c = 0; c < Cfg::NCH; ++c)
@@ -1078,7 +1086,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             } else if constexpr (MODE == 0 && GATED) {
                 if (EPI == EPI_GATED && !ok) break;
                 // h = act(first) * second, in the registers of the first
-                with_activation(ea.e, [&](auto act) {
+                with_activation(epi_flags & ACT_MASK, [&](auto act) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll

@@ -305,7 +305,7 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
         if (warp < Cfg::PROMO_WARPS && ok && n < p.N) {
             if constexpr (EPI == EPI_BIAS_ACT) {
                 const float bias = ea.e.bias ? bias_1(ea.e, n) : 0.0f;
-                with_activation(ea.e, [&](auto act) {
+                with_activation(ea.e.act, [&](auto act) {
 #pragma unroll
                     for (int t0 = 0; t0 < TW; t0 += 8) {               // eight residuals in flight
                         float r[8];
@@ -332,7 +332,7 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
         // partial sums to the CTA that finishes a row: [split][row of C][matrix][column] in its shared memory
         constexpr int PITCH = 512 * NW;               // bytes of a row
         const int per = (p.M + S - 1) / S;            // rows of C each CTA finishes
-        if (S > 1) ptx::cluster_wait();               // every CTA of the cluster runs
+        if (!GATED || S > 1) ptx::cluster_wait();     // every CTA of the cluster runs
         if (warp < Cfg::PROMO_WARPS && ok) {
             const uint32_t mine = red_base + static_cast<uint32_t>(rank * per * PITCH + ((warp & 3) * 32 + lane) * 4);
             int owner = row0 / per, local = row0 - owner * per;
@@ -351,7 +351,7 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                     }
                 }
         }
-        if (S > 1) ptx::cluster_sync();
+        if (!GATED || S > 1) ptx::cluster_sync();
         else __syncthreads();
         if (*abort_flag == 0u) {
             const int t0 = rank * per, rows = t0 + per < p.M ? per : p.M - t0;
