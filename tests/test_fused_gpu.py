@@ -274,3 +274,56 @@ def test_a_feed_forward_block(rows):
     gd = n @ Wg.double().t()
     plain = (gd * torch.sigmoid(gd) * (n @ Wu.double().t())) @ Wd.double().t()
     assert ((y.double() - s.double()) - plain).norm() <= 0.1 * plain.norm()
+
+
+@pytest.mark.parametrize("act,want", [
+    ("none", lambda x: x),
+    ("relu", lambda x: 0.0 if x < 0 else x),
+    ("silu", lambda x: x if x > 0 else 0.0),
+    ("gelu", lambda x: x if x > 0 else 0.0),
+    ("gelu_tanh", lambda x: x if x > 0 else 0.0)])
+@pytest.mark.parametrize("M,splits,tile", [(16, 1, f.SMALL_M), (64, 2, f.SMALL_M), (144, 1, 128), (144, 1, PAIR), (144, 2, 128)])
+def test_extreme_arguments_of_the_activations(act, want, M, splits, tile):
+    # sums are 0, so that the argument is the bias: infinities, NaN and magnitudes at which squares and exponentials overflow, each beside an
+    # ordinary value that must not be touched
+    N, K = 272, 256
+    A, a_s, _ = operand(M, K, 1, 1)
+    A.zero_()
+    B, b_s, _ = operand(N, K, 2, 128)
+    values = [float("inf"), 1.5, float("-inf"), 1.5, float("nan"), 1.5, 1e30, 1.5, -1e30, 1.5, 3e38, 1.5, -3e38, 1.5, -50.0, 1.5]
+    bias = torch.tensor((values * 17)[:N], device=DEV)
+    C = f.gemm_bias_act(A, B, a_s, b_s, M=M, N=N, K=K, bias=bias, activation=act, splits=splits, tile_n=tile).double()
+    ordinary = float(act64(torch.tensor(1.5, dtype=torch.float64), act))
+    for j, v in enumerate(values):
+        got = C[:, j::16]
+        if v == 1.5:
+            assert ((got - ordinary).abs() <= 2.0 ** -8 * ordinary).all()
+        elif v != v:
+            assert got.isnan().all()
+        elif act == "none" or want(v) != 0.0:
+            assert (got == torch.tensor(want(v), dtype=torch.float64).to(BF16).double()).all(), (v, got[0, 0])
+        else:
+            assert (got.abs() <= 1e-15).all(), (v, got[0, 0])           # the tail: below 40 * 2^-57
+
+
+def test_offsets_beyond_32_bits():
+    # C and the residual of 2.2e9 elements, the A operand of a wide product of 2.2e9 bytes: the last rows and columns are where they belong
+    M, N, K = 270336, 8192, 128
+    g = torch.Generator(device=DEV).manual_seed(1)
+    A = torch.randint(0x20, 0x40, (M * K,), dtype=torch.uint8, device=DEV, generator=g)
+    a_s = torch.rand(M, device=DEV, generator=g)
+    B, b_s, Bv = operand(N, K, 3, 128)
+    R = torch.randn(M, N, device=DEV, generator=g, dtype=BF16)
+    C = f.gemm_bias_act(A, B, a_s, b_s, M=M, N=N, K=K, residual=R, activation="relu")
+    q, sc = f.gemm_gated(A, B, B, a_s, b_s, b_s, M=M, N=N, K=K, activation="none", quantize=True)
+    f.last_device_status()
+    rows = torch.tensor([0, 1, M // 2 + 3, M - 17, M - 1], device=DEV)
+    Av = A.view(FP8).view(K, M)[:, rows].t().double() * a_s[rows, None].double()
+    x, err = product(Av, Bv)
+    y = x.clamp(min=0) + R[rows].double()
+    close_bf16(C[rows], y, 1.13 * err + U * y.abs())
+    h = (x * x).view(len(rows), N // 128, 128)
+    inv = sc.view(N // 128, M)[:, rows].t().double()
+    assert ((inv - h.amax(2) / 448.0).abs() <= 1e-5 * inv).all()
+    got = q.view(FP8).view(N, M)[:, rows].t().double().view(len(rows), N // 128, 128)
+    assert ((got * inv[:, :, None] - h).abs() <= h.amax(2, keepdim=True) * 2.0 ** -4 * 1.001).all()

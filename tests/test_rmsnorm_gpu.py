@@ -179,3 +179,41 @@ def test_feeds_the_product():
     # bf16's half step, and K + K / 128 fp32 roundings of the sum of magnitudes
     assert ((C.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + (K + 8) * 2.0 ** -24 * (A.abs() @ Bv.abs().t())).all()
     assert (C[rows:] == 0).all()
+
+
+def test_offsets_beyond_32_bits():
+    # 2.2e9 elements, in a slice of rows that are wider still
+    rows, K, wide = 264000, 8192, 8320
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(rows, wide, device=DEV, generator=g, dtype=BF16)[:, 64:64 + K]
+    r = torch.randn(rows, K, device=DEV, generator=g, dtype=BF16)
+    w = torch.ones(K, device=DEV)
+    pick = torch.tensor([0, 15, 16, rows // 2, rows - 33, rows - 1], device=DEV)
+    values, inv, s = want(x[pick], w, r[pick], 1e-6, 448.0)
+    q, sc, out = f.rmsnorm_quantize(x, w, residual=r, residual_out=r)
+    n = len(pick)
+    check_sum(out[pick], s)
+    got_inv = sc.view(K // 128, rows)[:, pick].t().double()
+    assert ((got_inv - inv[:n]).abs() <= SCALE_TOL * inv[:n]).all()
+    got = q.view(torch.float8_e4m3fn).view(K, rows)[:, pick].t().double()
+    half_step = torch.exp2(torch.floor(torch.log2(values[:n].abs().clamp(min=2.0 ** -6)))) * 2.0 ** -4
+    assert ((got - values[:n]).abs() <= half_step + VALUE_TOL * values[:n].abs()).all()
+
+
+def test_groups_at_odd_places_and_unaligned_bytes():
+    # 16 rows of a column leave together with the 16 before them where both lie in one aligned 32 bytes: every start and every number of
+    # groups, with outputs that begin on 16 but not on 32 bytes
+    K = 256
+    for rows in (16, 32, 48, 1000, 5000, 5016):
+        for lead in (0, 16):
+            x, w, r = make(rows, K, BF16, None, BF16, seed=rows)
+            M = (rows + 15) // 16 * 16
+            buf = torch.zeros(M * K + 64, dtype=torch.uint8, device=DEV)
+            q = buf[lead:lead + M * K]
+            sc = torch.zeros(M * K // 128, device=DEV)
+            assert q.data_ptr() % 32 == lead
+            assert f.lib().fp8bs_rmsnorm_quantize(x.data_ptr(), 1, K, None, 0, 0, None, w.data_ptr(), 1, q.data_ptr(), sc.data_ptr(), rows, K, 1e-6, 448.0,
+                                                  torch.cuda.current_stream().cuda_stream) == 0
+            values, inv, _ = want(x, w, None, 1e-6, 448.0)
+            check(q, sc, values, inv)
+            assert (buf[:lead] == 0).all() and (buf[lead + M * K:] == 0).all()
