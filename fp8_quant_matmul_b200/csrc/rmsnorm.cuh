@@ -271,27 +271,31 @@ rmsnorm_quantize_kernel(const NormParams p)
     const int groups = p.M / NORM_ROWS, clusters = static_cast<int>(gridDim.x) / C, id = static_cast<int>(blockIdx.x) / C;
     const int g0 = static_cast<int>(static_cast<long long>(groups) * id / clusters);
     const int g1 = static_cast<int>(static_cast<long long>(groups) * (id + 1) / clusters);
-    // 16 rows of x and of r, a copy per row, by warp 0
+    // 16 rows of x and of r, a copy per row; every warp issues its share (a copy holds the issuing warp for 80 cycles: all 32 in one warp
+    // took a third of a round), thread 0 says how many bytes there will be.
     auto request = [&](int g) {
         const int rows = min(NORM_ROWS, p.rows - g * NORM_ROWS);
-        if (rows < NORM_ROWS) {                      // the last 16 rows: zeros behind the last
-            for (uint32_t i = static_cast<uint32_t>(rows * width) * sizeof(X) + lane * 16; i < NORM_ROWS * width * sizeof(X); i += 512)
-                *reinterpret_cast<uint4*>(xs + i) = make_uint4(0u, 0u, 0u, 0u);
-            if (ADD)
-                for (uint32_t i = static_cast<uint32_t>(rows * width) * sizeof(RT) + lane * 16; i < NORM_ROWS * width * sizeof(RT); i += 512)
-                    *reinterpret_cast<uint4*>(rs + i) = make_uint4(0u, 0u, 0u, 0u);
-            __syncwarp();
+        if (threadIdx.x == 0) ptx::mbar_arrive_expect_tx(rows_bar, static_cast<uint32_t>(rows * cols * (sizeof(X) + (ADD ? sizeof(RT) : 0))));
+        const int copy = warp + lane * warps, i = copy & 15;           // copies 0-15: x, 16-31: r
+        if (copy < (ADD ? 32 : 16) && i < rows) {
+            const long long row = g * NORM_ROWS + i, col = rank * width;
+            if (copy < 16)
+                ptx::bulk_load(ptx::smem_u32(xs) + i * width * static_cast<int>(sizeof(X)), static_cast<const X*>(p.x) + row * p.ldx + col,
+                               static_cast<uint32_t>(cols * sizeof(X)), rows_bar);
+            else
+                ptx::bulk_load(ptx::smem_u32(rs) + i * width * static_cast<int>(sizeof(RT)), static_cast<const RT*>(p.r) + row * p.ldr + col,
+                               static_cast<uint32_t>(cols * sizeof(RT)), rows_bar);
         }
-        if (lane == 0) ptx::mbar_arrive_expect_tx(rows_bar, static_cast<uint32_t>(rows * cols * (sizeof(X) + (ADD ? sizeof(RT) : 0))));
         __syncwarp();
-        const long long row = g * NORM_ROWS + (lane & 15), col = rank * width;
-        if ((lane & 15) < rows) {
-            if (lane < 16)
-                ptx::bulk_load(ptx::smem_u32(xs) + (lane & 15) * width * static_cast<int>(sizeof(X)),
-                               static_cast<const X*>(p.x) + row * p.ldx + col, static_cast<uint32_t>(cols * sizeof(X)), rows_bar);
-            else if (ADD)
-                ptx::bulk_load(ptx::smem_u32(rs) + (lane & 15) * width * static_cast<int>(sizeof(RT)),
-                               static_cast<const RT*>(p.r) + row * p.ldr + col, static_cast<uint32_t>(cols * sizeof(RT)), rows_bar);
+        if (rows < NORM_ROWS) {                      // the last 16 rows: zeros behind the last, by warp 0 before its own sums
+            if (warp == 0) {
+                for (uint32_t b = static_cast<uint32_t>(rows * width) * sizeof(X) + lane * 16; b < NORM_ROWS * width * sizeof(X); b += 512)
+                    *reinterpret_cast<uint4*>(xs + b) = make_uint4(0u, 0u, 0u, 0u);
+                if (ADD)
+                    for (uint32_t b = static_cast<uint32_t>(rows * width) * sizeof(RT) + lane * 16; b < NORM_ROWS * width * sizeof(RT); b += 512)
+                        *reinterpret_cast<uint4*>(rs + b) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            __syncthreads();
         }
     };
     if (threadIdx.x == 0) {
@@ -305,7 +309,7 @@ rmsnorm_quantize_kernel(const NormParams p)
     if (C > 1) ptx::cluster_arrive();                // waited for before anything is sent to a peer: its barriers exist
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    if (warp == 0) request(g0);                      // clusters <= groups
+    request(g0);                                     // clusters <= groups
     if (C > 1) ptx::cluster_wait();
 
     auto cta_sum = [&](const float* ws, int row) {
@@ -346,7 +350,7 @@ rmsnorm_quantize_kernel(const NormParams p)
         // the round between keeps apart (for the peers': a CTA sends round n + 2 after it has round n + 1 from everybody).
         ok = __syncthreads_and(ok);
         if (!ok) break;
-        if (warp == 0 && g + 1 < g1) request(g + 1);
+        if (g + 1 < g1) request(g + 1);
         float total = 0.0f;
         if (C > 1) {
             const uint32_t bar = sums_bar + 8u * odd;
