@@ -2,10 +2,11 @@
 //   none   x                     silu       x / (1 + exp(-x))
 //   relu   x < 0 ? 0 : x         gelu       x (1 + erf(x / sqrt 2)) / 2
 //                                gelu_tanh  x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) / 2 = x / (1 + exp(-2 sqrt(2/pi) (x + 0.044715 x^3)))
-// silu and gelu_tanh are one function with two constants, x / (1 + 2^(x (a + b x^2))).  The special-function unit (four lanes per clock and
-// scheduler) is what activations cost: two values share one reciprocal (1 / d0 = d1 / (d0 d1)), 1.5 operations of that unit per value
-// instead of 2.  Errors (2^-22 of the exponential and of the reciprocal, and the argument's rounding) are below 1 % of a bf16 step where
-// the result is not itself negligible, and an output in 8 bits has its scale from the largest elements, where 2^(..) is next to nothing.
+// An activation is a few instructions for each of a thread's 64 or 128 columns, and the promotion warps (two per scheduler, with 88 registers
+// beside the sums) issue about one instruction in two cycles there: what counts is their number.  silu and bias on 4096 x 7168 x 512 took 41 us, and
+// 38 in a copy without any exponential or reciprocal; without an activation it takes 23.  Two values share one reciprocal (1 / d0 = d1 / (d0 d1)).
+// Errors (2^-22 of the exponential and of the reciprocal, and the argument's rounding) are below 1 % of a bf16 step where the result is not itself
+// negligible, and an output in 8 bits has its scale from the largest elements, where the exponential is next to nothing.
 // (In packed fp32 instructions the activations were no faster and the K loop of the pair kernel, which shares their registers, 17 %
 // slower, whichever was chosen at run time.)
 #pragma once
@@ -38,7 +39,7 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi)
     return r;
 }
 
-enum : int { ACT_NONE = 0, ACT_RELU = 1, ACT_LOGISTIC = 2, ACT_ERF = 3 };
+enum : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_ERF = 3, ACT_TANH = 4 };     // the numbers of FP8BS_ACT_*
 
 struct Epilogue {
     const void* bias;               // [N], NULL: none
@@ -49,7 +50,6 @@ struct Epilogue {
     float* scale_out;               // ... and its inverse scales [N / 128][M]
     int bias_is_bf16;
     int act;
-    float a, b, lowest;             // ACT_LOGISTIC: the constants, log2 e included; below `lowest` the function is -1e-16 at most
     float fp8_max;
 };
 
@@ -74,48 +74,58 @@ __device__ __forceinline__ float rcp_approx(float x)
     return y;
 }
 
-// x / (1 + 2^(x (a + b x^2))).  The argument of the exponential is held in a range (2^-6700 .. 2^60) in which nothing overflows and a NaN does not
-// reach the other value of the pair; the factor x keeps NaN and +infinity.
-__device__ __forceinline__ unsigned long long logistic_times_2(unsigned long long x, const Epilogue& e)
+// x0 / (1 + 2^z0), x1 / (1 + 2^z1); z up to 60, so that the product of the denominators does not overflow.
+__device__ __forceinline__ unsigned long long logistic_times_2(float x0, float x1, float z0, float z1)
 {
-    const float x0 = max_nan(f32x2_lo(x), e.lowest), x1 = max_nan(f32x2_hi(x), e.lowest);
-    const float t0 = fminf(x0, 40.0f), t1 = fminf(x1, 40.0f);
-    const float d0 = 1.0f + ex2_approx(t0 * fmaf(t0 * t0, e.b, e.a)), d1 = 1.0f + ex2_approx(t1 * fmaf(t1 * t1, e.b, e.a));
-    const float r = rcp_approx(d0 * d1);
+    const float d0 = 1.0f + ex2_approx(z0), d1 = 1.0f + ex2_approx(z1), r = rcp_approx(d0 * d1);
     return pack_f32x2(x0 * (r * d1), x1 * (r * d0));
 }
-
-// x (1 + erf(x / sqrt 2)) / 2 = max(x, 0) - |x| erfc(|x| / sqrt 2) / 2 with erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), t = 1 / (1 + p z): formula
+// silu.  Below -40 it stays at -40 / (1 + e^40) = -2e-16.  A NaN stays one, and out of the other value: its exponential is taken of something else.
+__device__ __forceinline__ unsigned long long silu_2(unsigned long long x)
+{
+    const float x0 = max_nan(f32x2_lo(x), -40.0f), x1 = max_nan(f32x2_hi(x), -40.0f);
+    constexpr float A = -1.4426950408889634f;
+    return logistic_times_2(x0, x1, fminf(x0 * A, 60.0f), fminf(x1 * A, 60.0f));
+}
+// gelu_tanh: x / (1 + 2^(A x + B x^3)).  Below -7.4 it stays there, at -2e-17; above 40 the exponential is 0 (and x^3 could overflow).
+__device__ __forceinline__ unsigned long long gelu_tanh_2(unsigned long long x)
+{
+    const float x0 = max_nan(f32x2_lo(x), -7.4f), x1 = max_nan(f32x2_hi(x), -7.4f);
+    const float t0 = fminf(x0, 40.0f), t1 = fminf(x1, 40.0f);                       // NaN: 40
+    constexpr float A = -1.4426950408889634f * 2.0f * 0.7978845608028654f, B = A * 0.044715f;
+    return logistic_times_2(x0, x1, t0 * fmaf(t0 * t0, B, A), t1 * fmaf(t1 * t1, B, A));
+}
+// gelu: x (1 + erf(x / sqrt 2)) / 2 = max(x, 0) - |x| erfc(|x| / sqrt 2) / 2 with erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), t = 1 / (1 + p z): formula
 // 7.1.26 of Abramowitz and Stegun, off by 1.5e-7 at most, that is 7.5e-8 |x| here; and the tail below 0 has no cancellation.  (CUDA's
 // erff in this place cost the K loop of the pair kernel 15 spilled registers.)
-__device__ __forceinline__ unsigned long long erf_times_2(unsigned long long x)
+__device__ __forceinline__ unsigned long long gelu_2(unsigned long long x)
 {
     const float x0 = f32x2_lo(x), x1 = f32x2_hi(x);
-    const float a0 = fminf(fabsf(x0), 100.0f), a1 = fminf(fabsf(x1), 100.0f);       // the tail is 0 there; NaN becomes 100
-    const float z0 = a0 * 0.70710678118654752f, z1 = a1 * 0.70710678118654752f;
-    const float p0 = fmaf(0.3275911f, z0, 1.0f), p1 = fmaf(0.3275911f, z1, 1.0f), r = rcp_approx(p0 * p1);
-    auto tail = [](float t, float z) {
-        const float poly = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-        return poly * t * ex2_approx(z * -1.4426950408889634f * z);
+    const float u0 = fminf(fabsf(x0), 100.0f), u1 = fminf(fabsf(x1), 100.0f);       // the tail is 0 there; NaN becomes 100
+    constexpr float P = 0.3275911f * 0.70710678118654752f, E = -0.5f * 1.4426950408889634f;
+    const float p0 = fmaf(P, u0, 1.0f), p1 = fmaf(P, u1, 1.0f), r = rcp_approx(p0 * p1);
+    auto tail = [](float t, float u) {                                              // -erfc / 2
+        const float poly = fmaf(t, fmaf(t, fmaf(t, fmaf(t, -0.5f * 1.061405429f, 0.5f * 1.453152027f), -0.5f * 1.421413741f), 0.5f * 0.284496736f),
+                                -0.5f * 0.254829592f);
+        return poly * t * ex2_approx(u * u * E);
     };
-    const float c0 = tail(r * p1, z0), c1 = tail(r * p0, z1);
-    // max(x, 0) keeps a NaN
-    return pack_f32x2(fmaf(a0 * -0.5f, c0, x0 < 0.0f ? 0.0f : x0), fmaf(a1 * -0.5f, c1, x1 < 0.0f ? 0.0f : x1));
+    return pack_f32x2(fmaf(u0, tail(r * p1, u0), max_nan(x0, 0.0f)), fmaf(u1, tail(r * p0, u1), max_nan(x1, 0.0f)));
 }
 template <int ACT>
-__device__ __forceinline__ unsigned long long activate_2(unsigned long long x, const Epilogue& e)
+__device__ __forceinline__ unsigned long long activate_2(unsigned long long x)
 {
-    if constexpr (ACT == ACT_RELU)                                   // a NaN stays one
-        return pack_f32x2(f32x2_lo(x) < 0.0f ? 0.0f : f32x2_lo(x), f32x2_hi(x) < 0.0f ? 0.0f : f32x2_hi(x));
-    else if constexpr (ACT == ACT_LOGISTIC) return logistic_times_2(x, e);
-    else if constexpr (ACT == ACT_ERF) return erf_times_2(x);
+    if constexpr (ACT == ACT_RELU) return pack_f32x2(max_nan(f32x2_lo(x), 0.0f), max_nan(f32x2_hi(x), 0.0f));       // a NaN stays one
+    else if constexpr (ACT == ACT_SILU) return silu_2(x);
+    else if constexpr (ACT == ACT_ERF) return gelu_2(x);
+    else if constexpr (ACT == ACT_TANH) return gelu_tanh_2(x);
     else return x;
 }
 // f(integral constant of the activation): one branch per call of this, not per element.
 template <class F>
 __device__ __forceinline__ void with_activation(int which, F f)
 {
-    if (which == ACT_LOGISTIC) f(std::integral_constant<int, ACT_LOGISTIC>{});
+    if (which == ACT_SILU) f(std::integral_constant<int, ACT_SILU>{});
+    else if (which == ACT_TANH) f(std::integral_constant<int, ACT_TANH>{});
     else if (which == ACT_ERF) f(std::integral_constant<int, ACT_ERF>{});
     else if (which == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
     else f(std::integral_constant<int, ACT_NONE>{});
@@ -140,8 +150,8 @@ __device__ __forceinline__ float4 activate_4(float4 v, const Epilogue& e)
 {
     unsigned long long a = pack_f32x2(v.x, v.y), b = pack_f32x2(v.z, v.w);
     with_activation(e.act, [&](auto act) {
-        a = activate_2<decltype(act)::value>(a, e);
-        b = activate_2<decltype(act)::value>(b, e);
+        a = activate_2<decltype(act)::value>(a);
+        b = activate_2<decltype(act)::value>(b);
     });
     return make_float4(f32x2_lo(a), f32x2_hi(a), f32x2_lo(b), f32x2_hi(b));
 }

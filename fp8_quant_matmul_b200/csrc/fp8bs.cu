@@ -943,15 +943,9 @@ static int fused_impl(const void* A, const void* B, const void* B2, const float*
     e.scale_out = out_scale;
     e.bias_is_bf16 = bias_is_bf16;
     e.fp8_max = fp8_max;
-    const double log2e = 1.4426950408889634, c = 2.0 * 0.7978845608028654;             // 2 sqrt(2 / pi)
-    switch (activation) {
-        case FP8BS_ACT_RELU: e.act = ACT_RELU; break;
-        case FP8BS_ACT_SILU: e.act = ACT_LOGISTIC; e.a = static_cast<float>(-log2e); e.b = 0.0f; e.lowest = -40.0f; break;
-        case FP8BS_ACT_GELU: e.act = ACT_ERF; break;
-        case FP8BS_ACT_GELU_TANH: e.act = ACT_LOGISTIC; e.a = static_cast<float>(-log2e * c); e.b = static_cast<float>(-log2e * c * 0.044715);
-            e.lowest = -7.4f; break;
-        default: e.act = ACT_NONE;
-    }
+    static_assert(FP8BS_ACT_NONE == ACT_NONE && FP8BS_ACT_RELU == ACT_RELU && FP8BS_ACT_SILU == ACT_SILU && FP8BS_ACT_GELU == ACT_ERF &&
+                  FP8BS_ACT_GELU_TANH == ACT_TANH, "the kernels' numbers of the activations");
+    e.act = activation;
     if (!gated) return launch_bias_act(cfg, tm, p, dev->sm_count, st, e);
     return fp8 ? launch_gated<EPI_GATED_FP8>(cfg, tm, p, dev->sm_count, st, e) : launch_gated<EPI_GATED>(cfg, tm, p, dev->sm_count, st, e);
 }

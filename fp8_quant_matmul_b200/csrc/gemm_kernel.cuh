@@ -865,7 +865,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         // What a tile has to know of its epilogue, in a register that the compiler takes as given: read from the parameters anew for every
         // tile it came from beyond the constant cache.
         int epi_flags = 0;
-        constexpr int HAS_BIAS = 4, BIAS_BF16 = 8, HAS_RESIDUAL = 16, ACT_MASK = 3;
+        constexpr int ACT_MASK = 7, HAS_BIAS = 8, BIAS_BF16 = 16, HAS_RESIDUAL = 32;
         if constexpr (EPI != EPI_NONE) {
             epi_flags = ea.e.act | (ea.e.bias ? HAS_BIAS : 0) | (ea.e.bias_is_bf16 ? BIAS_BF16 : 0) | (ea.e.residual ? HAS_RESIDUAL : 0);
             asm volatile("" : "+r"(epi_flags));
@@ -1060,7 +1060,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
                         for (int c = 0; c < Cfg::NCH; ++c)
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) acc[c][i] = activate_2<decltype(act)::value>(acc[c][i], ea.e);
+                            for (int i = 0; i < 16; ++i) acc[c][i] = activate_2<decltype(act)::value>(acc[c][i]);
                 });
                 if (residual_here()) {
                     ok = wait_bounded(residual_bar(pw), tcount & 1u, abort_flag, p.status, DS_TIMEOUT_STAGE_FULL);
@@ -1091,7 +1091,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const unsigned long long g = activate_2<decltype(act)::value>(acc[c][i], ea.e), up = acc[c + 2][i];
+                            const unsigned long long g = activate_2<decltype(act)::value>(acc[c][i]), up = acc[c + 2][i];
                             acc[c][i] = pack_f32x2(f32x2_lo(g) * f32x2_lo(up), f32x2_hi(g) * f32x2_hi(up));
                         }
                 });

@@ -315,7 +315,7 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
 #pragma unroll
                         for (int t = 0; t < 8; t += 2) {
                             const unsigned long long y =
-                                activate_2<decltype(act)::value>(ptx::add_f32x2(acc[(t0 + t) / 2], pack_f32x2(bias, bias)), ea.e);
+                                activate_2<decltype(act)::value>(ptx::add_f32x2(acc[(t0 + t) / 2], pack_f32x2(bias, bias)));
                             __nv_bfloat16* c = p.C + static_cast<size_t>(row0 + t0 + t) * p.N + n;
                             if (row0 + t0 + t < p.rows) *c = __float2bfloat16_rn(f32x2_lo(y) + r[t]);
                             if (row0 + t0 + t + 1 < p.rows) c[p.N] = __float2bfloat16_rn(f32x2_hi(y) + r[t + 1]);
