@@ -146,36 +146,54 @@ __device__ __forceinline__ float bias_1(const Epilogue& e, int n)
     return e.bias_is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(e.bias)[n]) : __ldg(static_cast<const float*>(e.bias) + n);
 }
 
-__device__ __forceinline__ float4 activate_4(float4 v, const Epilogue& e)
+// The activation of R groups of four values.
+template <int R>
+__device__ __forceinline__ void activate_4(float4 (&v)[R], const Epilogue& e)
 {
-    unsigned long long a = pack_f32x2(v.x, v.y), b = pack_f32x2(v.z, v.w);
     with_activation(e.act, [&](auto act) {
-        a = activate_2<decltype(act)::value>(a);
-        b = activate_2<decltype(act)::value>(b);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const unsigned long long a = activate_2<decltype(act)::value>(pack_f32x2(v[i].x, v[i].y));
+            const unsigned long long b = activate_2<decltype(act)::value>(pack_f32x2(v[i].z, v[i].w));
+            v[i] = make_float4(f32x2_lo(a), f32x2_hi(a), f32x2_lo(b), f32x2_hi(b));
+        }
     });
-    return make_float4(f32x2_lo(a), f32x2_hi(a), f32x2_lo(b), f32x2_hi(b));
 }
-// act(gate) * up
-__device__ __forceinline__ float4 gate_4(float4 gate, float4 up, const Epilogue& e)
+// gate = act(gate) * up
+template <int R>
+__device__ __forceinline__ void gate_4(float4 (&gate)[R], const float4 (&up)[R], const Epilogue& e)
 {
-    const float4 g = activate_4(gate, e);
-    return make_float4(g.x * up.x, g.y * up.y, g.z * up.z, g.w * up.w);
+    activate_4(gate, e);
+#pragma unroll
+    for (int i = 0; i < R; ++i) gate[i] = make_float4(gate[i].x * up[i].x, gate[i].y * up[i].y, gate[i].z * up[i].z, gate[i].w * up[i].w);
 }
 
-// act(v + bias) + residual of four neighbouring columns of row m.
-__device__ __forceinline__ float4 finish_4(float4 v, const Epilogue& e, int m, int n)
+// The residual of columns n .. n + 3 of rows m, m + step, ..; those from `rows` on are left at 0.
+template <int R>
+__device__ __forceinline__ void residual_4(uint2 (&r)[R], const Epilogue& e, int m, int step, int rows, int n)
 {
-    uint2 r = make_uint2(0u, 0u);
-    if (e.residual) r = *reinterpret_cast<const uint2*>(e.residual + m * e.ldr + n);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        r[i] = make_uint2(0u, 0u);
+        if (e.residual && m + i * step < rows) r[i] = *reinterpret_cast<const uint2*>(e.residual + (m + i * step) * e.ldr + n);
+    }
+}
+// act(v + bias) + residual of columns n .. n + 3 of R rows.
+template <int R>
+__device__ __forceinline__ void finish_4(float4 (&v)[R], const uint2 (&r)[R], const Epilogue& e, int n)
+{
     if (e.bias) {
         const float4 b = bias_4(e, n);
-        v = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
+#pragma unroll
+        for (int i = 0; i < R; ++i) v[i] = make_float4(v[i].x + b.x, v[i].y + b.y, v[i].z + b.z, v[i].w + b.w);
     }
-    v = activate_4(v, e);
-    if (e.residual)
-        v = make_float4(v.x + __uint_as_float(r.x << 16), v.y + __uint_as_float(r.x & 0xffff0000u), v.z + __uint_as_float(r.y << 16),
-                        v.w + __uint_as_float(r.y & 0xffff0000u));
-    return v;
+    activate_4(v, e);
+    if (e.residual) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            v[i] = make_float4(v[i].x + __uint_as_float(r[i].x << 16), v[i].y + __uint_as_float(r[i].x & 0xffff0000u),
+                               v[i].z + __uint_as_float(r[i].y << 16), v[i].w + __uint_as_float(r[i].y & 0xffff0000u));
+    }
 }
 
 // The factor that takes a group whose largest magnitude is amax to 8 bits, and the inverse scale to be stored (as in

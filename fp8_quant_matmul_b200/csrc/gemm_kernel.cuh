@@ -378,6 +378,16 @@ __global__ void wait_timeout_selftest_kernel(unsigned int* status, long long lim
     (void)ok;
 }
 
+// The cluster reduction (MODE 2): rows of one column quad in the buffer of the CTA that finishes them, [split][quad][row] of float4.  As many as
+// the largest share; odd, so that neighbouring quads of a row are in other banks.
+__host__ __device__ constexpr int sums_pitch(int splits) { return ((127 + splits) / splits) | 1; }
+__host__ __device__ constexpr bool cluster_sums_fit(int bn, int bytes)
+{
+    for (int splits = 2; splits <= 8; ++splits)
+        if (splits * (bn / 4) * sums_pitch(splits) * 16 > bytes) return false;
+    return true;
+}
+
 template <int BN, int CG, int MODE, int EPI = EPI_NONE>
 __global__ void __launch_bounds__(TileCfg<BN, CG>::THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -398,9 +408,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     static_assert(MODE != 3 || CG == 1, "stream-K is built for single-CTA tiles");
     constexpr bool RESIDENT = (MODE == 4);              // both K blocks of a tile kept in TMEM (K <= 256)
     static_assert(!RESIDENT || (CG == 1 && BN == 256), "the short-K mode uses 256-wide single-CTA tiles");
-    // MODE 2: fp32 partial tile of this CTA, rows padded by 16 bytes so that a warp's 32 rows hit distinct banks
-    constexpr int PART_PITCH = BN * 4 + 16;
-    static_assert(MODE != 2 || 128 * PART_PITCH <= STAGES * Cfg::STAGE_BYTES, "partial tile must fit in the stage area");
+    constexpr int ABSMAX_BYTES = EPI == EPI_GATED_FP8 ? 1024 : 0;
+    static_assert(MODE != 2 || cluster_sums_fit(BN, STAGES * Cfg::STAGE_BYTES + Cfg::STG_BYTES - ABSMAX_BYTES),
+                  "partial sums must fit in the stage buffers and the staging area behind them");
+    constexpr int RED_ROWS = 4;                    // float4 that a thread of the cluster reduction has in flight
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw);
@@ -528,85 +539,132 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     // from each CTA's B slab (slab r holds the tile's columns 128 r ..), which come out as the part's two pieces.
     auto col_of = [](int g, int q) { return CG == 2 ? g * 64 + q * 128 : g * Cfg::COLS + q * 64; };
 
-    // MODE 2: the cluster reduction.  Gated it runs inside the promotion warps' branch: its sums of two products would spill in the 64
-    // registers that the code after the branches has to make do with (and spills leave the SM: shared memory takes all of L1).  15 us.
-    auto cluster_meet = [&]() {
-        __syncthreads();                 // this CTA's partial tile is complete ...
-        ptx::cluster_sync();             // ... and so are those of the other K ranges of the tile
-    };
+    // MODE 2: the cluster reduction.  Each CTA finishes a share of the tile's rows.  Once every CTA's MMAs are done (the stage buffers are
+    // free), the sums go from the registers straight into the stage buffers of the CTA that finishes their row, [split][column quad][row]: a
+    // warp's store is 32 rows of 16 bytes, one behind the other.  After a second meeting all reads are local.  (Left in the writer's shared
+    // memory and fetched from there row by row, the reduction took 1.9 us longer with two splits of a 256-wide tile; with more fetches in flight it was
+    // slower still with three.  What is left of it: 1.9 us, three splits 3.0, for the way between the SMs, about 30 bytes a ns each, and 2 for the rest.)
+    // It runs inside the promotion warps' branch: the sums of several rows in flight would spill in the 64 registers that the code after
+    // the branches has to make do with (and spills leave the SM: shared memory takes all of L1).
+    auto first_row = [&](int split) { return (128 * split) / p.splits; };        // of a CTA's share
+    auto row_pitch = [&]() { return sums_pitch(p.splits); };
     auto cluster_reduce = [&]() {
         if (*abort_flag != 0u) return;
         const int S = p.splits;
         const int my = static_cast<int>(ptx::cluster_ctarank());     // = this CTA's split index
         int tile, m0, n0, kb0, kb1;
         decode(static_cast<int>(blockIdx.x), tile, m0, n0, kb0, kb1);
-        // the rows this CTA finishes (gated fp8: in sixteens)
-        const int r0 = EPI == EPI_GATED_FP8 ? 16 * ((8 * my) / S) : (128 * my) / S;
-        const int r1 = EPI == EPI_GATED_FP8 ? 16 * ((8 * (my + 1)) / S) : (128 * (my + 1)) / S;
-        uint32_t peer[8];
+        const int r0 = first_row(my), r1 = first_row(my + 1), pitch = row_pitch();
+        // sum[0][i]: the sum of column quad `quad` + i QSTEP and row `row` + i RSTEP (the last row again behind it); sum[1], gated: 16 quads on.  Splits in
+        // fixed order: bit-deterministic.
+        auto sum_at = [&](auto& sum, int quad, int row, auto qstep, auto rstep) {
+            constexpr int R = sizeof(sum[0]) / sizeof(float4), NQ = sizeof(sum) / sizeof(sum[0]);
+            int at[R];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) peer[s] = ptx::mapa(stage_base, static_cast<uint32_t>(s < S ? s : 0));
-        auto sum_at = [&](int row, int c) {                         // splits in fixed order: bit-deterministic
-            const uint32_t off = static_cast<uint32_t>(row * PART_PITCH + c * 4);
-            float4 v[8];
+            for (int i = 0; i < R; ++i) {
+                const int r = row + i * decltype(rstep)::value;
+                at[i] = (quad + i * decltype(qstep)::value) * pitch + (r < r1 ? r : r1 - 1) - r0;
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
-                if (s < S) v[s] = ptx::ld_shared_cluster_v4(peer[s] + off);
-            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-                if (s < S) { sum.x += v[s].x; sum.y += v[s].y; sum.z += v[s].z; sum.w += v[s].w; }
-            return sum;
-        };
-        if constexpr (GATED) {
-            // A warp takes a row, a lane four columns.  Partial tiles are laid out [column group][first | second][64].  Bytes are collected
-            // [column][row] in the staging area, from where 16 rows of a column leave at a time: stored one by one (32 sectors per instruction)
-            // they took 6 us more than bf16 rows on 192 x 2304 x 1024.
-            constexpr int PITCH = 64 + 4;                    // two CTAs at least share the rows; words of a column, other banks for the next
-            static_assert(128 * PITCH <= Cfg::STG_BYTES, "staging area");
-            const int c = lane * 4, part = (c >> 6) * 128 + (c & 63);
+                for (int q = 0; q < NQ; ++q) sum[q][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
 #pragma unroll 1
-            for (int row = r0 + warp - 4; row < r1; row += Cfg::PROMO_WARPS) {
-                const float4 g = sum_at(row, part), up = sum_at(row, part + 64);
-                const float4 h = gate_4(g, up, ea.e);
-                const int m = m0 + row;
-                if constexpr (EPI == EPI_GATED_FP8) {
-                    const float amax = warp_absmax_nan(max_nan(max_nan(fabsf(h.x), fabsf(h.y)), max_nan(fabsf(h.z), fabsf(h.w))));
-                    float inverse;
-                    const float f = scale_factor(amax, ea.e.fp8_max, inverse);
-                    if (lane == 0 && m < p.M) ea.e.scale_out[static_cast<size_t>(n0 >> 7) * p.M + m] = inverse;
-                    const uint32_t lo = cvt_e4m3x2(h.x * f, h.y * f), hi = cvt_e4m3x2(h.z * f, h.w * f);
-                    uint8_t* at = stg_ptr + c * PITCH + (row - r0);
-                    at[0] = static_cast<uint8_t>(lo);
-                    at[PITCH] = static_cast<uint8_t>(lo >> 8);
-                    at[2 * PITCH] = static_cast<uint8_t>(hi);
-                    at[3 * PITCH] = static_cast<uint8_t>(hi >> 8);
-                } else if (m < p.rows && n0 + c < p.N) {
-                    *reinterpret_cast<uint2*>(p.C + static_cast<size_t>(m) * p.N + n0 + c) = make_uint2(pack_bf16x2(h.x, h.y), pack_bf16x2(h.z, h.w));
-                }
+            for (int s = 0; s < S; ++s) {
+                const float4* part = reinterpret_cast<const float4*>(aligned) + s * (BN / 4) * pitch;
+                float4 v[NQ][R];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int i = 0; i < R; ++i) v[q][i] = part[at[i] + q * 16 * pitch];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int i = 0; i < R; ++i) {
+                        sum[q][i].x += v[q][i].x; sum[q][i].y += v[q][i].y; sum[q][i].z += v[q][i].z; sum[q][i].w += v[q][i].w;
+                    }
             }
-            if constexpr (EPI == EPI_GATED_FP8) {
+        };
+        // Partial tiles of a gated product are laid out [column group][first | second][64].
+        if constexpr (EPI == EPI_GATED_FP8) {
+            // A lane takes a row, a warp some of its columns: the warps of a row tell one another its largest magnitude, and a column's bytes
+            // leave as 32 neighbouring ones.  (A warp per row, with a reduction over its lanes and two reciprocals for each, and the bytes collected
+            // in shared memory on their way: 1.5 us more on 192 x 2304 x 1024 with two splits.)
+            auto rows_by_lane = [&](auto warps) {
+                constexpr int W = decltype(warps)::value, Q = 32 / W;             // warps per row, column quads of each
+                const int pw = warp - 4, row = r0 + (pw / W) * 32 + lane, w = pw % W, m = m0 + row;
+                float4 h[Q];
+                float amax = 0.0f;
+#pragma unroll
+                for (int q = 0; q < Q; q += RED_ROWS) {
+                    float4 sum[2][RED_ROWS];
+                    const int quad = w * Q + q;
+                    sum_at(sum, (quad >> 4) * 32 + (quad & 15), row, std::integral_constant<int, 1>{}, std::integral_constant<int, 0>{});
+                    gate_4(sum[0], sum[1], ea.e);
+#pragma unroll
+                    for (int i = 0; i < RED_ROWS; ++i) {
+                        h[q + i] = sum[0][i];
+                        amax = max_nan(amax, max_nan(max_nan(fabsf(h[q + i].x), fabsf(h[q + i].y)), max_nan(fabsf(h[q + i].z), fabsf(h[q + i].w))));
+                    }
+                }
+                float* const most = reinterpret_cast<float*>(stg_ptr + Cfg::STG_BYTES - ABSMAX_BYTES) + (pw / W) * 32 + lane;
+                most[w * (256 / W)] = amax;
                 asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(Cfg::PROMO_THREADS) : "memory");
-                for (int idx = static_cast<int>(threadIdx.x) - 128; idx < 128 * ((r1 - r0) >> 4); idx += Cfg::PROMO_THREADS) {
-                    const int k = idx & 127, r = (idx >> 7) * 16;
-                    const uint32_t* from = reinterpret_cast<const uint32_t*>(stg_ptr + k * PITCH + r);
-                    if (m0 + r0 + r < p.M)                   // M is a multiple of 16: all 16 rows or none
-                        *reinterpret_cast<uint4*>(ea.e.q_out + static_cast<size_t>(n0 + k) * p.M + m0 + r0 + r) =
-                            make_uint4(from[0], from[1], from[2], from[3]);
+#pragma unroll
+                for (int i = 0; i < W; ++i) amax = max_nan(amax, most[i * (256 / W)]);
+                if (row >= r1 || m >= p.M) return;
+                float inverse;
+                const float f = scale_factor(amax, ea.e.fp8_max, inverse);
+                if (w == 0) ea.e.scale_out[static_cast<size_t>(n0 >> 7) * p.M + m] = inverse;
+                uint8_t* to = ea.e.q_out + static_cast<size_t>(n0 + w * Q * 4) * p.M + m;
+#pragma unroll
+                for (int i = 0; i < Q; ++i) {
+                    const uint32_t lo = cvt_e4m3x2(h[i].x * f, h[i].y * f), hi = cvt_e4m3x2(h[i].z * f, h[i].w * f);
+                    to[0] = static_cast<uint8_t>(lo);
+                    to[p.M] = static_cast<uint8_t>(lo >> 8);
+                    to[2 * static_cast<size_t>(p.M)] = static_cast<uint8_t>(hi);
+                    to[3 * static_cast<size_t>(p.M)] = static_cast<uint8_t>(hi >> 8);
+                    to += 4 * static_cast<size_t>(p.M);
+                }
+            };
+            if (S < 4) rows_by_lane(std::integral_constant<int, 4>{});            // up to 64 rows
+            else rows_by_lane(std::integral_constant<int, 8>{});                  // up to 32
+        } else if constexpr (GATED) {
+            // a warp takes a row, a lane four columns
+            constexpr int R = RED_ROWS / 2;
+            const int c = lane * 4, quad = (lane >> 4) * 32 + (lane & 15);
+#pragma unroll 1
+            for (int row = r0 + warp - 4; row < r1; row += R * Cfg::PROMO_WARPS) {
+                float4 sum[2][R];
+                sum_at(sum, quad, row, std::integral_constant<int, 0>{}, std::integral_constant<int, Cfg::PROMO_WARPS>{});
+                gate_4(sum[0], sum[1], ea.e);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const int m = m0 + row + i * Cfg::PROMO_WARPS;
+                    if (row + i * Cfg::PROMO_WARPS < r1 && m < p.rows && n0 + c < p.N)
+                        *reinterpret_cast<uint2*>(p.C + static_cast<size_t>(m) * p.N + n0 + c) =
+                            make_uint2(pack_bf16x2(sum[0][i].x, sum[0][i].y), pack_bf16x2(sum[0][i].z, sum[0][i].w));
                 }
             }
-        }
-        const int items = GATED ? 0 : (r1 - r0) * (BN / 4);
-        for (int idx = static_cast<int>(threadIdx.x) - 128; idx < items; idx += Cfg::PROMO_THREADS) {
-            const int row = r0 + idx / (BN / 4), c4 = idx % (BN / 4);
-            float4 sum = sum_at(row, c4 * 4);
-            const int m = m0 + row, n = n0 + c4 * 4;
-            if (m < p.rows && n < p.N) {
-                if constexpr (EPI == EPI_BIAS_ACT) sum = finish_4(sum, ea.e, m, n);
-                uint2 q;
-                q.x = pack_bf16x2(sum.x, sum.y);
-                q.y = pack_bf16x2(sum.z, sum.w);
-                *reinterpret_cast<uint2*>(p.C + static_cast<size_t>(m) * p.N + n) = q;
+        } else {
+            // a thread takes four columns of every STEP-th row
+            constexpr int R = RED_ROWS, STEP = Cfg::PROMO_THREADS / (BN / 4);
+            const int t = static_cast<int>(threadIdx.x) - 128, c = (t % (BN / 4)) * 4, n = n0 + c;
+            const int end = m0 + r1 < p.rows ? m0 + r1 : p.rows;
+#pragma unroll 1
+            for (int row = r0 + t / (BN / 4); row < r1; row += R * STEP) {
+                float4 sum[1][R];
+                [[maybe_unused]] uint2 res[R];
+                if constexpr (EPI == EPI_BIAS_ACT) residual_4(res, ea.e, m0 + row, STEP, n < p.N ? end : 0, n);
+                sum_at(sum, t % (BN / 4), row, std::integral_constant<int, 0>{}, std::integral_constant<int, STEP>{});
+                if (n < p.N) {
+                    if constexpr (EPI == EPI_BIAS_ACT) finish_4(sum[0], res, ea.e, n);
+#pragma unroll
+                    for (int i = 0; i < R; ++i) {
+                        const int m = m0 + row + i * STEP;
+                        if (m < end)
+                            *reinterpret_cast<uint2*>(p.C + static_cast<size_t>(m) * p.N + n) =
+                                make_uint2(pack_bf16x2(sum[0][i].x, sum[0][i].y), pack_bf16x2(sum[0][i].z, sum[0][i].w));
+                    }
+                }
             }
         }
     };
@@ -844,7 +902,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
         }
         __syncwarp();
-        if constexpr (MODE == 2 && GATED) cluster_meet();
+        if constexpr (MODE == 2) {
+            ptx::cluster_sync();
+            ptx::cluster_sync();
+        }
     } else {
         // -------------------------------------------------------- promotion + epilogue ------
         ptx::setmaxnreg_inc<216>();
@@ -861,6 +922,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         uint32_t ait = 0;
         uint32_t tcount = 0;                     // MODE 4: tiles done by this CTA
         bool ok = true;
+        [[maybe_unused]] bool met = false;       // MODE 2: the first of the two meetings is behind this CTA
         PROF_DECL(w_tfull); PROF_DECL(t_fma); PROF_DECL(t_epi);
         // What a tile has to know of its epilogue, in a register that the compiler takes as given: read from the parameters anew for every
         // tile it came from beyond the constant cache.
@@ -1227,12 +1289,19 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     ok = wait_bounded(tfull_bar(NH - 1, (ait - 1) % NBUF), ((ait - 1) / NBUF) & 1u, abort_flag, p.status, DS_TIMEOUT_TMEM_FULL);
                     ok = __all_sync(0xffffffffu, ok);
                 }
+                ptx::cluster_sync();
+                met = true;
                 if (ok) {
-                    float4* dst = reinterpret_cast<float4*>(aligned + row_in_tile * PART_PITCH + grp * Cfg::COLS * 4);
+                    const int my = static_cast<int>(ptx::cluster_ctarank());
+                    int owner = (row_in_tile * p.splits) >> 7;
+                    while (first_row(owner + 1) <= row_in_tile) ++owner;        // the quotient is the owner or the one before
+                    const int at = (my * (BN / 4) + grp * (Cfg::COLS / 4)) * row_pitch() + row_in_tile - first_row(owner);
+                    const uint32_t step = static_cast<uint32_t>(row_pitch()) * 16u;
+                    const uint32_t dst = ptx::mapa(stage_base, static_cast<uint32_t>(owner)) + static_cast<uint32_t>(at) * 16u;
 #pragma unroll
                     for (int j = 0; j < Cfg::COLS / 4; ++j)
-                        dst[j] = make_float4(f32x2_lo(acc[j / 8][(2 * j) % 16]), f32x2_hi(acc[j / 8][(2 * j) % 16]),
-                                             f32x2_lo(acc[j / 8][(2 * j + 1) % 16]), f32x2_hi(acc[j / 8][(2 * j + 1) % 16]));
+                        ptx::st_shared_cluster_v4(dst + j * step, make_float4(f32x2_lo(acc[j / 8][(2 * j) % 16]), f32x2_hi(acc[j / 8][(2 * j) % 16]),
+                                                                              f32x2_lo(acc[j / 8][(2 * j + 1) % 16]), f32x2_hi(acc[j / 8][(2 * j + 1) % 16])));
                 }
             } else {
                 // ---- split-K: publish this K range's partial sums ----
@@ -1318,21 +1387,18 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         // C must have been read out of shared memory before the CTA goes away
         if (ptx::elect_one()) ptx::tma_store_wait_read<0>();
         __syncwarp();
-        if constexpr (MODE == 2 && GATED) {
-            cluster_meet();
+        if constexpr (MODE == 2) {
+            if (!met) ptx::cluster_sync();
+            ptx::cluster_sync();
             cluster_reduce();
         }
     }
 
-    if constexpr (MODE == 2 && !GATED) {
-        cluster_meet();
-        if (warp >= 4) cluster_reduce();
-    }
 
     // ---------------------------------------------------------------- common exit -----
     ptx::tc_fence_before_sync();
     __syncthreads();
-    if constexpr (CG == 2 || MODE == 2) ptx::cluster_sync();   // nothing remote may touch this CTA after it has left
+    if constexpr (CG == 2) ptx::cluster_sync();   // nothing remote may touch this CTA after it has left (MODE 2: nothing does after the second meeting)
     if (warp == 1) {
         __syncwarp();
         ptx::tc_fence_after_sync();

@@ -370,10 +370,12 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                         if (s < S) { sum.x += v[s].x; sum.y += v[s].y; sum.z += v[s].z; sum.w += v[s].w; }
                     return sum;
                 };
-                float4 sum = sum_at(0);
+                float4 sums[1] = {sum_at(0)};
                 if constexpr (GATED) {
-                    sum = gate_4(sum, sum_at(1), ea.e);
+                    const float4 up[1] = {sum_at(1)};
+                    gate_4(sums, up, ea.e);
                 }
+                const float4& sum = sums[0];
                 if constexpr (EPI == EPI_GATED_FP8) {
                     // a warp's lanes are the 128 columns of row t
                     const float amax = warp_absmax_nan(max_nan(max_nan(fabsf(sum.x), fabsf(sum.y)), max_nan(fabsf(sum.z), fabsf(sum.w))));
@@ -387,7 +389,11 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                     dst[2 * p.M] = static_cast<uint8_t>(hi);
                     dst[3 * p.M] = static_cast<uint8_t>(hi >> 8);
                 } else if (n0 + c < p.N && t0 + t < p.rows) {
-                    if constexpr (EPI == EPI_BIAS_ACT) sum = finish_4(sum, ea.e, t0 + t, n0 + c);
+                    if constexpr (EPI == EPI_BIAS_ACT) {
+                        uint2 r[1];
+                        residual_4(r, ea.e, t0 + t, 1, p.rows, n0 + c);
+                        finish_4(sums, r, ea.e, n0 + c);
+                    }
                     uint2 q;
                     q.x = pack_bf16x2(sum.x, sum.y);
                     q.y = pack_bf16x2(sum.z, sum.w);

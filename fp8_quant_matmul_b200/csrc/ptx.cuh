@@ -218,14 +218,9 @@ __device__ __forceinline__ void st_async_f32(uint32_t cluster_addr, float v, uin
                  : "memory");
 }
 // 16 bytes from the shared memory of any CTA of the cluster (address from mapa).
-__device__ __forceinline__ float4 ld_shared_cluster_v4(uint32_t cluster_addr)
+__device__ __forceinline__ void st_shared_cluster_v4(uint32_t cluster_addr, float4 v)
 {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(cluster_addr)
-                 : "memory");
-    return v;
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 // Arrive on an mbarrier that may live in another CTA of the cluster (shared::cluster address).
 // Default semantics on purpose: a cluster-scope release costs several hundred cycles per arrive, and the
