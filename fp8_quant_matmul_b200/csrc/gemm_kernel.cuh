@@ -15,9 +15,9 @@
 //                 added in split order 0..S-1, so the result does not depend on timing (replaces
 //                 k_large_kernel, mn_small.hip:10-137, which instead shrinks the tile to get more
 //                 blocks).  MODE 2 (S <= 8): the S CTAs of a tile form a
-//                 thread-block cluster, each leaves its fp32 partial tile in its own shared memory,
-//                 and after a cluster barrier every CTA reduces 128/S rows straight out of its
-//                 peers' shared memory (DSMEM): no workspace, no atomics.  MODE 1 (any S, also pair
+//                 thread-block cluster, each sends its fp32 sums into the shared memory of the CTA
+//                 that finishes their row (DSMEM), 128/S rows each, and after a cluster barrier
+//                 every CTA adds up what it was sent: no workspace, no atomics.  MODE 1 (any S, also pair
 //                 tiles): partial sums go to an fp32 workspace and whoever finishes a tile last adds
 //                 them.
 //           3 stream-K: the K blocks of all tiles are dealt out evenly over the CTAs; a tile that
@@ -124,6 +124,10 @@ struct GemmParams {
 // first product beside the same 64 of the second, and a promotion thread owns both.  A single CTA loads both slabs, hands the tile
 // over as one part, and its column group g takes columns 64 g .. of each slab.  A tile is exactly one scale block of h wide: its
 // two column groups exchange their rows' largest magnitudes through shared memory.
+// Bound by the K loop, as the product alone is; the epilogue's instructions are not hidden (the promotion warps issue them between two K
+// loops), its bytes are.  Measured: bias, gelu_tanh and residual on 6144 x 4608 x 7168 177-180 us (gemm() 160 in a short run, 182 at the power limit);
+// gated 4096 x 2048 x 7168 to bytes 103 (gemm() on 4096 x 4096 x 7168 98), 192 x 2304 x 7168 in three splits 19.8 (gemm() on 192 x 4608 x 7168
+// 14.8 on 128-wide tiles, which a gated scale block does not fit).
 enum : int { EPI_NONE = 0, EPI_BIAS_ACT = 1, EPI_GATED = 2, EPI_GATED_FP8 = 3 };
 constexpr int EPI_BIAS_BYTES = 8 * 512;              // per promotion warp: the bias of its columns (gated fp8: [column group][row] magnitudes)
 constexpr int epi_smem(int epi) { return epi == EPI_NONE ? 0 : EPI_BIAS_BYTES; }
@@ -408,9 +412,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     static_assert(MODE != 3 || CG == 1, "stream-K is built for single-CTA tiles");
     constexpr bool RESIDENT = (MODE == 4);              // both K blocks of a tile kept in TMEM (K <= 256)
     static_assert(!RESIDENT || (CG == 1 && BN == 256), "the short-K mode uses 256-wide single-CTA tiles");
-    constexpr int ABSMAX_BYTES = EPI == EPI_GATED_FP8 ? 1024 : 0;
-    static_assert(MODE != 2 || cluster_sums_fit(BN, STAGES * Cfg::STAGE_BYTES + Cfg::STG_BYTES - ABSMAX_BYTES),
-                  "partial sums must fit in the stage buffers and the staging area behind them");
+    static_assert(MODE != 2 || cluster_sums_fit(BN, STAGES * Cfg::STAGE_BYTES), "partial sums must fit in the stage buffers");
     constexpr int RED_ROWS = 4;                    // float4 that a thread of the cluster reduction has in flight
 
     extern __shared__ uint8_t smem_raw[];
@@ -605,7 +607,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                         amax = max_nan(amax, max_nan(max_nan(fabsf(h[q + i].x), fabsf(h[q + i].y)), max_nan(fabsf(h[q + i].z), fabsf(h[q + i].w))));
                     }
                 }
-                float* const most = reinterpret_cast<float*>(stg_ptr + Cfg::STG_BYTES - ABSMAX_BYTES) + (pw / W) * 32 + lane;
+                float* const most = reinterpret_cast<float*>(stg_ptr + (epi_base - stg_base)) + (pw / W) * 32 + lane;       // [warp of a row][row]
                 most[w * (256 / W)] = amax;
                 asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(Cfg::PROMO_THREADS) : "memory");
 #pragma unroll

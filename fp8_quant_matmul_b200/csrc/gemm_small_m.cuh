@@ -23,7 +23,8 @@ namespace fp8bs {
 
 // EPI: the fused epilogues of gemm_kernel.cuh.  Gated: a K block brings 128 columns of both matrices (a stage of 32 KB of weights, one CTA
 // per SM), a promotion thread owns one column of both products, and all partial sums go through shared memory, so that a warp
-// then holds the 128 columns of a row: one scale block.
+// then holds the 128 columns of a row: one scale block.  16 x 2048 x 7168 to bytes: 9.5-10.3 us for 29.5 MB of weights (4.6 us at the copy's rate);
+// on average an SM is at work for 12000 of the launch's 26000 cycles.
 template <int T, int EPI = EPI_NONE>
 struct SmallMCfg {
     static constexpr bool GATED = (EPI == EPI_GATED || EPI == EPI_GATED_FP8);
