@@ -906,6 +906,15 @@ static int gemm_impl(const void* A, const void* B, const float* a_scale, const f
     return launch_config(cfg, tm, p, dev->sm_count, st);
 }
 
+// Whether an output overlaps an input [rows, n] with a pitch of ld elements in any other way than element on element (an output [rows, n]
+// without gaps that starts where the input does, in the same type): the rows of one are read after others of the other are written.
+static bool overlaps_badly(const void* out, int out_size, const void* in, int in_size, long long rows, long long n, long long ld)
+{
+    const char *o = static_cast<const char*>(out), *i = static_cast<const char*>(in);
+    if (o == i && out_size == in_size && (ld == n || rows == 1)) return false;
+    return o < i + ((rows - 1) * ld + n) * in_size && i < o + rows * n * out_size;
+}
+
 // The fused calls.  B2 NULL: one product with bias, activation and residual; else the gated pair, in 8 bits where out_scale is given.
 static int fused_impl(const void* A, const void* B, const void* B2, const float* a_scale, const float* b_scale, const float* b2_scale, void* out,
                       float* out_scale, int M, int N, int K, int rows, const void* bias, int bias_is_bf16, int activation, const void* residual,
@@ -923,6 +932,7 @@ static int fused_impl(const void* A, const void* B, const void* B2, const float*
     if (off(A, 16) || off(B, 16) || off(B2, 16) || off(out, 16) || off(a_scale, 16) || off(b_scale, 4) || off(b2_scale, 4) || off(out_scale, 4) ||
         off(bias, 16) || off(residual, 16) || (residual && ldr % 8 != 0))
         return FP8BS_ERR_ALIGN;
+    if (residual && overlaps_badly(out, 2, residual, 2, rows, N, ldr)) return FP8BS_ERR_ARG;
     DeviceInfo* dev = nullptr;
     const int dev_rc = device_setup(&dev);
     Config cfg{};
@@ -1791,6 +1801,9 @@ int fp8bs_rmsnorm_quantize(const void* X, int x_is_bf16, long long ldx, const vo
     if (residual && (off(residual) || off(residual_out) || ldr % (r_is_bf16 ? 8 : 4) != 0)) return FP8BS_ERR_ALIGN;
     if (off(A_out) || (reinterpret_cast<uintptr_t>(a_scale_out) & 3u)) return FP8BS_ERR_ALIGN;
     if (!(fp8_max > 0.0f) || fp8_max > 448.0f || !(eps >= 0.0f)) return FP8BS_ERR_ARG;
+    const int x_size = x_is_bf16 ? 2 : 4, r_size = r_is_bf16 ? 2 : 4;
+    if (residual && (overlaps_badly(residual_out, r_size, residual, r_size, rows, K, ldr) || overlaps_badly(residual_out, r_size, X, x_size, rows, K, ldx)))
+        return FP8BS_ERR_ARG;
     const long long groups = (static_cast<long long>(rows) + 15) / 16;
     if (groups * NORM_MAX_CLUSTER > 0x7fffffff) return FP8BS_ERR_SHAPE;
     DeviceInfo* dev = nullptr;

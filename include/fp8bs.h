@@ -141,7 +141,7 @@ int fp8bs_gemm_ex(const void* A, const void* B, const float* a_scale, const floa
  *   bias        [N], bf16 (bias_is_bf16 != 0) or fp32, 16-byte aligned; NULL: none
  *   activation  FP8BS_ACT_*
  *   residual    [rows, N] bf16 with a row pitch of ld_residual elements (>= N, a multiple of 8), 16-byte aligned; NULL: none.  It may be
- *               C itself (ld_residual = N); it must not overlap C otherwise.
+ *               C itself (ld_residual = N); any other overlap with C is refused.
  *   splits      0 = let the library choose; 1..8 = K cut over a cluster of that many CTAs
  *   tile_n      0 = choose; 128; 256 (splits 0 or > 1); 256 | FP8BS_TILE_PAIR (splits 0 or 1); FP8BS_SMALL_M (M <= 64)
  * Needs no workspace.  Asynchronous on `stream`. */
@@ -257,7 +257,7 @@ int fp8bs_quantize_block(const void* W, int w_is_bf16, void* B_out, float* b_sca
  *     a_scale_out[m + Mp*kb] = 1 / scale,  A_out[m + Mp*k] = e4m3fn(clamp(y * scale)),  scale as in fp8bs_quantize_rowwise
  * The norm sees s before it is rounded to residual_out.  X is [rows, K] with a row pitch of ldx elements, residual (may be NULL:
  * no addition, residual_out is not written) [rows, K] with a pitch of ldr, residual_out [rows, K] without gaps; residual_out may be
- * the residual itself or X itself if that has no gaps (ldr or ldx = K), and must not overlap them otherwise.  Each of X, residual
+ * the residual itself, or X itself if it has the same type, without gaps (ldr or ldx = K); any other overlap with them is refused.  Each of X, residual
  * and weight [K] is bf16 (its flag != 0) or fp32.  Any rows >= 1: Mp is rows rounded up to a multiple of 16, and the rows behind
  * the last are written as zeros (scale fp8_max / 1e-12), so that one token is an operand of 16 rows.  A row that holds a NaN or an
  * infinity gets NaN bytes and scales where torch's arithmetic has NaN.  K a multiple of 128 (rows of more

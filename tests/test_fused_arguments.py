@@ -14,7 +14,7 @@ def p(v):
     return ctypes.c_void_p(v) if v else None
 
 
-def bias_act(A=0x1000, B=0x2000, a=0x3000, b=0x4000, C=0x5000, M=128, N=256, K=512, rows=128, bias=0x6000, bb=0, act=0, r=0x7000, ldr=256, splits=0,
+def bias_act(A=0x1000, B=0x2000, a=0x3000, b=0x4000, C=0x500000, M=128, N=256, K=512, rows=128, bias=0x6000, bb=0, act=0, r=0x7000, ldr=256, splits=0,
              tile=0):
     return f.lib().fp8bs_gemm_bias_act(p(A), p(B), p(a), p(b), p(C), M, N, K, rows, p(bias), bb, act, p(r), ldr, splits, tile, None)
 
@@ -29,6 +29,7 @@ def gated(A=0x1000, G=0x2000, U=0x2800, a=0x3000, g=0x4000, u=0x4800, H=0x5000, 
     (dict(M=0, rows=0), -2), (dict(N=0), -2), (dict(K=100), -2), (dict(M=120, rows=120), -3), (dict(N=200), -3), (dict(rows=0), -2), (dict(rows=129), -2),
     (dict(A=0x1008), -3), (dict(B=0x2001), -3), (dict(C=0x5002), -3), (dict(a=0x3004), -3), (dict(b=0x4002), -3), (dict(bias=0x6004), -3),
     (dict(r=0x7008), -3), (dict(ldr=260), -3), (dict(ldr=248), -5),
+    (dict(r=0x500000, ldr=512), -5), (dict(r=0x500010), -5), (dict(r=0x4fffe0), -5), (dict(r=0x500000 - 127 * 1024 - 512 + 16, ldr=512), -5),
     (dict(act=-1), -5), (dict(act=5), -5), (dict(splits=-1), -5), (dict(splits=5), -5), (dict(K=2048, splits=9), -5),
     (dict(tile=192), -5), (dict(tile=256, splits=1), -5), (dict(tile=PAIR, splits=2), -5), (dict(tile=128 | f.TILE_PAIR), -5),
     (dict(tile=f.SMALL_M), -5), (dict(tile=f.SMALL_M | 256, M=64, rows=64), -5), (dict(tile=128 | f.SPLIT_WORKSPACE), -5), (dict(tile=f.STREAM_K), -5),
@@ -57,6 +58,9 @@ def test_without_a_device_valid_calls_are_an_error():
     if torch.cuda.is_available():
         pytest.skip("a GPU is present")
     for kw in (dict(), dict(tile=128), dict(tile=PAIR), dict(splits=2, tile=256), dict(M=64, rows=60, tile=f.SMALL_M), dict(M=16, rows=1, r=0, ldr=0, bias=0)):
+        assert bias_act(**kw) == -6
+    # the residual is C, or lies in front of it or behind it
+    for kw in (dict(r=0x500000), dict(r=0x500000, ldr=512, rows=1), dict(r=0x500000 + 0x10000), dict(r=0x500000 - 0x10000)):
         assert bias_act(**kw) == -6
     for kw in (dict(), dict(tile=256), dict(tile=PAIR), dict(splits=3), dict(s=0, N=208, fp8_max=0.0), dict(M=16, rows=2, splits=4)):
         assert gated(**kw) == -6

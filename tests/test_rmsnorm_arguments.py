@@ -27,6 +27,9 @@ def c_call(X=0x1000, xb=1, ldx=256, r=0x2000, rb=1, ldr=256, ro=0x3000, w=0x4000
     (dict(ldx=128), -5), (dict(ldr=252), -5), (dict(ldx=260), -3), (dict(ldr=257), -3), (dict(ldx=258, xb=0), -3),
     (dict(X=0x1004), -3), (dict(X=0x1008, xb=0), -3), (dict(r=0x2002), -3), (dict(ro=0x3008, rb=0), -3), (dict(w=0x4004), -3),
     (dict(A=0x5008), -3), (dict(s=0x6002), -3),
+    # the sum over the residual or X, but not element on element: other pitches, types, places
+    (dict(ro=0x2000, ldr=512), -5), (dict(ro=0x1000, ldx=512), -5), (dict(ro=0x1000, xb=0), -5), (dict(ro=0x1000, rb=0, ldr=256, r=0x8000), -5),
+    (dict(ro=0x2010), -5), (dict(ro=0x17f0), -5), (dict(ro=0x27f0), -5),
     (dict(fp8_max=0.0), -5), (dict(fp8_max=449.0), -5), (dict(fp8_max=float("nan")), -5), (dict(eps=-1.0), -5), (dict(eps=float("nan")), -5),
 ], ids=lambda v: str(v).replace(" ", "") if isinstance(v, dict) else "")
 def test_library_refuses(kw, code):
@@ -40,3 +43,5 @@ def test_without_a_device_it_is_an_error():
         pytest.skip("a GPU is present")
     assert c_call() == -6
     assert c_call(r=0, ro=0, ldr=0) == -6          # no residual: its arguments are not looked at
+    assert c_call(ro=0x2000) == -6 and c_call(ro=0x1000) == -6 and c_call(ro=0x1000, ldx=512, rows=1) == -6       # in place
+    assert c_call(ro=0x2800) == -6 and c_call(ro=0x1800) == -6                                                     # side by side

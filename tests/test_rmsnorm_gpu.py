@@ -217,3 +217,18 @@ def test_groups_at_odd_places_and_unaligned_bytes():
             values, inv, _ = want(x, w, None, 1e-6, 448.0)
             check(q, sc, values, inv)
             assert (buf[:lead] == 0).all() and (buf[lead + M * K:] == 0).all()
+
+
+def test_the_first_call_of_a_shape_may_be_captured():
+    """Shapes that no other test here uses: what the library asks the driver about them is asked under capture."""
+    f.rmsnorm_quantize(torch.ones(16, 128, device="cuda"), torch.ones(128, device="cuda"))
+    for K, xt in ((128 * 13, F32), (128 * 97, BF16)):
+        x = torch.randn(37, K, device="cuda", generator=torch.Generator("cuda").manual_seed(K)).to(xt)
+        w = torch.ones(K, device="cuda")
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            q, s = f.rmsnorm_quantize(x, w)
+        g.replay()
+        torch.cuda.synchronize()
+        q2, s2 = f.rmsnorm_quantize(x, w)
+        assert torch.equal(q, q2) and torch.equal(s, s2)
