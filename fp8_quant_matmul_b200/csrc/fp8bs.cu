@@ -125,22 +125,6 @@ static int prepare_small_m()
     return FP8BS_OK;
 }
 
-template <int EPI>
-static int prepare_fused_small_m()
-{
-    int rc;
-    if ((rc = prepare_small_m<16, EPI>()) || (rc = prepare_small_m<32, EPI>())) return rc;
-    return prepare_small_m<64, EPI>();
-}
-
-template <int EPI>
-static int prepare_gated()
-{
-    int rc;
-    if ((rc = prepare_kernel<256, 2, 0, EPI>()) || (rc = prepare_kernel<256, 1, 0, EPI>()) || (rc = prepare_kernel<256, 1, 2, EPI>())) return rc;
-    return prepare_fused_small_m<EPI>();
-}
-
 template <bool BLOCK_SCALE>
 static int prepare_quantize()
 {
@@ -187,10 +171,7 @@ static int device_setup(DeviceInfo** out)
             (rc = prepare_kernel<128, 1, 3>()) || (rc = prepare_kernel<256, 1, 3>()) ||
             (rc = prepare_kernel<256, 1, 4>()) || (rc = prepare_small_m<16>()) ||
             (rc = prepare_small_m<32>()) || (rc = prepare_small_m<64>()) ||
-            (rc = prepare_quantize<false>()) || (rc = prepare_quantize<true>()) ||
-            (rc = prepare_kernel<128, 1, 0, EPI_BIAS_ACT>()) || (rc = prepare_kernel<256, 2, 0, EPI_BIAS_ACT>()) ||
-            (rc = prepare_kernel<128, 1, 2, EPI_BIAS_ACT>()) || (rc = prepare_kernel<256, 1, 2, EPI_BIAS_ACT>()) ||
-            (rc = prepare_fused_small_m<EPI_BIAS_ACT>()) || (rc = prepare_gated<EPI_GATED>()) || (rc = prepare_gated<EPI_GATED_FP8>())) {
+            (rc = prepare_quantize<false>()) || (rc = prepare_quantize<true>())) {
             d.status = rc;
             return rc;
         }
@@ -693,29 +674,54 @@ static int launch_small_m(const TensorMaps& tm, const GemmParams& p, cudaStream_
     return launch_clusters(gemm_small_m_kernel<T, EPI>, p.n_tiles * p.splits, p.splits, Cfg::THREADS, Cfg::SMEM_BYTES, stream, tm.A, tm.B, p, up, e);
 }
 
-template <int EPI>
-static int launch_fused_small_m(const TensorMaps& tm, const GemmParams& p, cudaStream_t st, const EpiArg<EPI>& e)
+// The kernels with a fused epilogue are set up by the first call that uses them: with all of them in device_setup the first gemm() of a
+// process took 19 ms instead of 7.
+template <int (*PREPARE)()>
+static int prepared(const DeviceInfo* dev)
 {
-    return p.M <= 16 ? launch_small_m<16, EPI>(tm, p, st, e) : p.M <= 32 ? launch_small_m<32, EPI>(tm, p, st, e) : launch_small_m<64, EPI>(tm, p, st, e);
+    static std::atomic<bool> done[MAX_DEVICES];
+    std::atomic<bool>& d = done[dev - g_dev];
+    if (d.load(std::memory_order_acquire)) return FP8BS_OK;
+    const int rc = PREPARE();
+    if (rc == FP8BS_OK) d.store(true, std::memory_order_release);
+    return rc;
+}
+template <int BN, int CG, int MODE, int EPI>
+static int launch_fused(const DeviceInfo* dev, const TensorMaps& tm, const GemmParams& p, cudaStream_t st, const EpiArg<EPI>& e)
+{
+    const int rc = prepared<prepare_kernel<BN, CG, MODE, EPI>>(dev);
+    return rc ? rc : launch<BN, CG, MODE, EPI>(tm, p, dev->sm_count, st, e);
+}
+template <int T, int EPI>
+static int launch_fused_small_m(const DeviceInfo* dev, const TensorMaps& tm, const GemmParams& p, cudaStream_t st, const EpiArg<EPI>& e)
+{
+    const int rc = prepared<prepare_small_m<T, EPI>>(dev);
+    return rc ? rc : launch_small_m<T, EPI>(tm, p, st, e);
+}
+template <int EPI>
+static int launch_fused_few_rows(const DeviceInfo* dev, const TensorMaps& tm, const GemmParams& p, cudaStream_t st, const EpiArg<EPI>& e)
+{
+    return p.M <= 16 ? launch_fused_small_m<16, EPI>(dev, tm, p, st, e) : p.M <= 32 ? launch_fused_small_m<32, EPI>(dev, tm, p, st, e)
+                                                                                    : launch_fused_small_m<64, EPI>(dev, tm, p, st, e);
 }
 
 // The fused calls: bias, activation and residual on 128-wide and pair tiles, or in the cluster reduction ...
-static int launch_bias_act(const Config& c, const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t st, const Epilogue& epilogue)
+static int launch_bias_act(const DeviceInfo* dev, const Config& c, const TensorMaps& tm, const GemmParams& p, cudaStream_t st, const Epilogue& epilogue)
 {
     constexpr int EPI = EPI_BIAS_ACT;
     const EpiArg<EPI> e{epilogue};
-    if (c.mode == 5) return launch_fused_small_m<EPI>(tm, p, st, e);
-    if (c.mode == 2) return c.tile_n == 256 ? launch<256, 1, 2, EPI>(tm, p, sm_count, st, e) : launch<128, 1, 2, EPI>(tm, p, sm_count, st, e);
-    return c.cg == 2 ? launch<256, 2, 0, EPI>(tm, p, sm_count, st, e) : launch<128, 1, 0, EPI>(tm, p, sm_count, st, e);
+    if (c.mode == 5) return launch_fused_few_rows<EPI>(dev, tm, p, st, e);
+    if (c.mode == 2) return c.tile_n == 256 ? launch_fused<256, 1, 2, EPI>(dev, tm, p, st, e) : launch_fused<128, 1, 2, EPI>(dev, tm, p, st, e);
+    return c.cg == 2 ? launch_fused<256, 2, 0, EPI>(dev, tm, p, st, e) : launch_fused<128, 1, 0, EPI>(dev, tm, p, st, e);
 }
 // ... and the gated pair of products, on tiles of 2 x 128 columns.
 template <int EPI>
-static int launch_gated(const Config& c, const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t st, const Epilogue& epilogue)
+static int launch_gated(const DeviceInfo* dev, const Config& c, const TensorMaps& tm, const GemmParams& p, cudaStream_t st, const Epilogue& epilogue)
 {
     const EpiArg<EPI> e{epilogue};
-    if (c.mode == 5) return launch_fused_small_m<EPI>(tm, p, st, e);
-    if (c.mode == 2) return launch<256, 1, 2, EPI>(tm, p, sm_count, st, e);
-    return c.cg == 2 ? launch<256, 2, 0, EPI>(tm, p, sm_count, st, e) : launch<256, 1, 0, EPI>(tm, p, sm_count, st, e);
+    if (c.mode == 5) return launch_fused_few_rows<EPI>(dev, tm, p, st, e);
+    if (c.mode == 2) return launch_fused<256, 1, 2, EPI>(dev, tm, p, st, e);
+    return c.cg == 2 ? launch_fused<256, 2, 0, EPI>(dev, tm, p, st, e) : launch_fused<256, 1, 0, EPI>(dev, tm, p, st, e);
 }
 
 // How many clusters of `cluster` CTAs with `warps` warps of the norm kernel run at once: asked once per device, type and shape.
@@ -961,8 +967,8 @@ static int fused_impl(const void* A, const void* B, const void* B2, const float*
     static_assert(FP8BS_ACT_NONE == ACT_NONE && FP8BS_ACT_RELU == ACT_RELU && FP8BS_ACT_SILU == ACT_SILU && FP8BS_ACT_GELU == ACT_ERF &&
                   FP8BS_ACT_GELU_TANH == ACT_TANH, "the kernels' numbers of the activations");
     e.act = activation;
-    if (!gated) return launch_bias_act(cfg, tm, p, dev->sm_count, st, e);
-    return fp8 ? launch_gated<EPI_GATED_FP8>(cfg, tm, p, dev->sm_count, st, e) : launch_gated<EPI_GATED>(cfg, tm, p, dev->sm_count, st, e);
+    if (!gated) return launch_bias_act(dev, cfg, tm, p, st, e);
+    return fp8 ? launch_gated<EPI_GATED_FP8>(dev, cfg, tm, p, st, e) : launch_gated<EPI_GATED>(dev, cfg, tm, p, st, e);
 }
 
 // ---------------------------------------------------------------------------------------

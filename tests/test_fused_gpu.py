@@ -7,6 +7,9 @@ the exponential multiplies by at most 20 before the result is below 2^-19 of x; 
 bf16: half a step, 2^-8 of the value.  8 bits: half a step of e4m3 (2^-4 of the value's binade, 2^-10 below 2^-6); the scale is as far off as
 the largest element of its group, and 4 roundings."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -20,6 +23,7 @@ DEV = "cuda"
 PAIR = 256 | f.TILE_PAIR
 U = 2.0 ** -24
 ACT_ERR = 2.0 ** -19
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def operand(rows, K, seed, rows_per_group, std=1.0, live=None):
@@ -327,3 +331,32 @@ def test_offsets_beyond_32_bits():
     assert ((inv - h.amax(2) / 448.0).abs() <= 1e-5 * inv).all()
     got = q.view(FP8).view(N, M)[:, rows].t().double().view(len(rows), N // 128, 128)
     assert ((got * inv[:, :, None] - h).abs() <= h.amax(2, keepdim=True) * 2.0 ** -4 * 1.001).all()
+
+
+FIRST_CALLS = """
+import torch, fp8_quant_matmul_b200 as f
+K, N = 256, 256
+one = torch.ones(4096, device="cuda")
+A, B = (torch.full((n * K,), 0x38, dtype=torch.uint8, device="cuda") for n in (160, N))       # ones
+f.gemm(A, B, one, one, M=16, N=N, K=K)
+torch.cuda.synchronize()
+outs = []
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    for M in (16, 160):
+        for splits in (0, 2):
+            outs.append(f.gemm_bias_act(A, B, one, one, M=M, N=N, K=K, activation="relu", splits=splits))
+            outs.append(f.gemm_gated(A, B, B, one, one, one, M=M, N=N, K=K, activation="none", splits=splits))
+            outs.append(f.gemm_gated(A, B, B, one, one, one, M=M, N=N, K=K, activation="none", quantize=True, splits=splits)[1])
+g.replay()
+f.last_device_status()
+for i in range(0, len(outs), 3):
+    assert (outs[i] == 256).all() and (outs[i + 1] == 65536).all() and torch.allclose(outs[i + 2], one[:1] * 65536 / 448)
+print("captured")
+"""
+
+
+def test_the_first_fused_calls_of_a_process_may_be_captured():
+    """A process of its own: each kernel is set up by the first call that uses it, here under capture."""
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stdout + done.stderr
