@@ -27,6 +27,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libfp8bs.so")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",
+    "--compress-mode=none",     # 13 MB instead of 5, and the first call of a process takes 7 ms instead of 13
 ]
 
 

@@ -674,8 +674,8 @@ static int launch_small_m(const TensorMaps& tm, const GemmParams& p, cudaStream_
     return launch_clusters(gemm_small_m_kernel<T, EPI>, p.n_tiles * p.splits, p.splits, Cfg::THREADS, Cfg::SMEM_BYTES, stream, tm.A, tm.B, p, up, e);
 }
 
-// The kernels with a fused epilogue are set up by the first call that uses them: with all of them in device_setup the first gemm() of a
-// process took 19 ms instead of 7.
+// The kernels with a fused epilogue are set up by the first call that uses them: all of them in device_setup add 0.8 ms to the first call of a
+// process, whichever that is (7 ms).
 template <int (*PREPARE)()>
 static int prepared(const DeviceInfo* dev)
 {
