@@ -333,6 +333,58 @@ def test_offsets_beyond_32_bits():
     assert ((got * inv[:, :, None] - h).abs() <= h.amax(2, keepdim=True) * 2.0 ** -4 * 1.001).all()
 
 
+
+@pytest.mark.parametrize("splits", [2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("M,rows", [(80, 67), (128, 128), (272, 257)])
+def test_every_number_of_splits(splits, M, rows):
+    """The shares of a tile's rows are of other sizes and start at other places for each; nothing around the results is touched."""
+    N, K = 256, 1152
+    (A, G, P, a_s, g_s, p_s), (Av, Gv, Pv) = gated_operands(M, rows, N, K)
+    pad, stream = 256, torch.cuda.current_stream().cuda_stream
+    q = torch.full((M * N + 2 * pad,), 0xAB, dtype=torch.uint8, device=DEV)
+    sc = torch.full((M * 2 + 2 * pad,), -7.0, device=DEV)
+    rc = f.lib().fp8bs_gemm_gated(A.data_ptr(), G.data_ptr(), P.data_ptr(), a_s.data_ptr(), g_s.data_ptr(), p_s.data_ptr(), q[pad:].data_ptr(), sc[pad:].data_ptr(),
+                                  M, N, K, rows, f.ACTIVATIONS["silu"], 448.0, splits, 256, stream)
+    assert rc == 0
+    f.last_device_status()
+    for buf, n, fill in ((q, M * N, 0xAB), (sc, M * 2, -7.0)):
+        assert (buf[:pad] == fill).all() and (buf[pad + n:] == fill).all()
+    h, err = gated_want(Av, Gv, Pv, "silu")
+    inv = sc[pad:pad + M * 2].view(2, M).t().double()
+    amax, e = (v.view(M, 2, 128).abs().amax(2) for v in (h, err))
+    assert ((inv - amax.clamp(min=1e-12) / 448.0).abs() <= 1.01 * e / 448.0 + 4 * U * inv).all()
+    exact = (h.view(M, 2, 128) / inv[:, :, None]).view(M, N)
+    got = q[pad:pad + M * N].view(FP8).view(N, M).t().double()
+    half_step = torch.exp2(torch.floor(torch.log2(exact.abs().clamp(min=2.0 ** -6)))) * 2.0 ** -4
+    assert ((got - exact).abs() <= half_step + (1.01 * err.view(M, 2, 128) / inv[:, :, None]).view(M, N) + 2.0 ** -20 * exact.abs()).all()
+    H = torch.full((rows + 1, N), 7.0, dtype=BF16, device=DEV)
+    f.gemm_gated(A, G, P, a_s, g_s, p_s, M=M, N=N, K=K, rows=rows, H=H[:rows], splits=splits, tile_n=256)
+    close_bf16(H[:rows], h[:rows], err[:rows])
+    assert (H[rows] == 7.0).all()
+    product_of_one, e1 = product(Av, Gv)
+    for tile in (128, 256):
+        C = torch.full((rows + 1, N), 7.0, dtype=BF16, device=DEV)
+        f.gemm_bias_act(A, G, a_s, g_s, C[:rows], M=M, N=N, K=K, rows=rows, splits=splits, tile_n=tile)
+        close_bf16(C[:rows], product_of_one[:rows], e1[:rows])
+        assert (C[rows] == 7.0).all()
+
+
+def test_one_matrix_in_both_places():
+    """The same tensor as both weights of the gated product, in two calls on two streams at once."""
+    M, N, K = 272, 256, 640
+    (A, G, _, a_s, g_s, _), (Av, Gv, _) = gated_operands(M, M, N, K)
+    h, err = gated_want(Av, Gv, Gv, "relu")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(f.gemm_gated(A, G, G, a_s, g_s, g_s, M=M, N=N, K=K, activation="relu", splits=1 + i % 3))
+    torch.cuda.synchronize()
+    for H in outs:
+        close_bf16(H, h, err)
+
+
 FIRST_CALLS = """
 import torch, fp8_quant_matmul_b200 as f
 K, N = 256, 256

@@ -83,7 +83,7 @@ def test_every_mix_of_types_on_column_slices(xt, rt, wt):
         check_sum(out[2], s)
 
 
-@pytest.mark.parametrize("K", [768, 9216])
+@pytest.mark.parametrize("K", [768, 9216, 17408])
 @pytest.mark.parametrize("which", ["residual", "x"])
 def test_the_sum_in_place(K, which):
     x, w, r = make(37, K, BF16, BF16, BF16, seed=9)
@@ -232,3 +232,14 @@ def test_the_first_call_of_a_shape_may_be_captured():
         torch.cuda.synchronize()
         q2, s2 = f.rmsnorm_quantize(x, w)
         assert torch.equal(q, q2) and torch.equal(s, s2)
+
+
+@pytest.mark.parametrize("K", [1280, 20480])
+def test_x_is_its_own_residual(K):
+    x, w, _ = make(45, K, F32, None, F32, seed=21)
+    values, inv, s = want(x, w, x, 1e-6, 448.0)
+    a = f.rmsnorm_quantize(x, w, residual=x)
+    check(a[0], a[1], values, inv)
+    b = f.rmsnorm_quantize(x, w, residual=x, residual_out=x)             # all three one tensor
+    assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(a, b))
+    check_sum(x, s)
