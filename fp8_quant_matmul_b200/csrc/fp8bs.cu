@@ -732,7 +732,7 @@ static int norm_clusters(int device, int cluster, int warps, int smem, int* out)
     std::atomic<int>& slot = known[device][cluster][warps];
     int n = slot.load(std::memory_order_relaxed);
     if (n == 0) {
-        CUDA_TRY(cudaFuncSetAttribute(rmsnorm_quantize_kernel<X, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_SMEM_LIMIT + NORM_FIXED_SMEM));
+        CUDA_TRY(cudaFuncSetAttribute(rmsnorm_quantize_kernel<X, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_SMEM_LIMIT));
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(cluster * 64), 1, 1);
         cfg.blockDim = dim3(static_cast<unsigned>(32 * warps), 1, 1);
@@ -752,6 +752,25 @@ static int norm_clusters(int device, int cluster, int warps, int smem, int* out)
     return FP8BS_OK;
 }
 
+// Rows of the norm's input in boxes of 16 x 128.
+template <class T>
+static int encode_norm_map(CUtensorMap* tm, const void* base, int rows, int K, long long ld)
+{
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * sizeof(T)};
+    const cuuint32_t box[2] = {128u, static_cast<cuuint32_t>(NORM_ROWS)};
+    const cuuint32_t estr[2] = {1u, 1u};
+    const CUresult r = g_encode_tiled(tm, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base), dims, strides, box,
+                                      estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        tl_last_cuda_error = static_cast<int>(r);
+        return FP8BS_ERR_CUDA;
+    }
+    return FP8BS_OK;
+}
+
 template <class X, class R>
 static int launch_rmsnorm(NormParams p, const DeviceInfo* dev, cudaStream_t st)
 {
@@ -762,17 +781,20 @@ static int launch_rmsnorm(NormParams p, const DeviceInfo* dev, cudaStream_t st)
     const int KB = p.K / 128, groups = p.M / NORM_ROWS;
     const int warps = ceil_div(KB, std::min(ceil_div(KB, element == 8 ? 6 : NORM_WARPS), NORM_MAX_CLUSTER));
     const int cluster = std::min(ceil_div(KB, warps), NORM_MAX_CLUSTER);         // every CTA has a block at least
-    const long long buffers = static_cast<long long>(NORM_ROWS) * 128 * warps * element;
-    if (warps > NORM_MOST_WARPS || buffers > NORM_SMEM_LIMIT)
+    const long long smem = static_cast<long long>(NORM_ROWS) * 128 * warps * element + norm_fixed_smem(cluster * warps);
+    if (warps > NORM_MOST_WARPS || smem > NORM_SMEM_LIMIT)
         return launch_grid(rmsnorm_quantize_long_kernel<X, R>, dim3(static_cast<unsigned>(groups * NORM_MAX_CLUSTER), 1, 1), NORM_MAX_CLUSTER,
                            32 * NORM_WARPS, 0, st, p);
-    const int smem = static_cast<int>(buffers) + NORM_FIXED_SMEM;
     int most = 0;
-    const int rc = norm_clusters<X, R>(static_cast<int>(dev - g_dev), cluster, warps, smem, &most);
+    int rc = norm_clusters<X, R>(static_cast<int>(dev - g_dev), cluster, warps, static_cast<int>(smem), &most);
     if (rc) return rc;
+    CUtensorMap x_map{}, r_map{};
+    if ((rc = encode_norm_map<X>(&x_map, p.x, p.rows, p.K, p.ldx))) return rc;
+    if constexpr (!std::is_void<R>::value)
+        if ((rc = encode_norm_map<R>(&r_map, p.r, p.rows, p.K, p.ldr))) return rc;
     p.cluster = cluster;
-    return launch_grid(rmsnorm_quantize_kernel<X, R>, dim3(static_cast<unsigned>(std::min(groups, most) * cluster), 1, 1), cluster, 32 * warps, smem,
-                       st, p);
+    return launch_grid(rmsnorm_quantize_kernel<X, R>, dim3(static_cast<unsigned>(std::min(groups, most) * cluster), 1, 1), cluster, 32 * warps,
+                       static_cast<int>(smem), st, x_map, r_map, p);
 }
 
 static int launch_config(const Config& c, const TensorMaps& tm, const GemmParams& p, int sm_count, cudaStream_t st)

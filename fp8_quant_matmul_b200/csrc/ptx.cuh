@@ -210,14 +210,13 @@ __device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, flo
 {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
-// The same without waiting for it to land: the four bytes are counted on `cluster_bar`, a barrier of the receiving CTA.
-__device__ __forceinline__ void st_async_f32(uint32_t cluster_addr, float v, uint32_t cluster_bar)
+// 16 bytes without waiting for them to land: they are counted on `cluster_bar`, a barrier of the receiving CTA.
+__device__ __forceinline__ void st_async_v4(uint32_t cluster_addr, float4 v, uint32_t cluster_bar)
 {
-    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];"
-                 ::"r"(cluster_addr), "r"(__float_as_uint(v)), "r"(cluster_bar)
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+                 ::"r"(cluster_addr), "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(__float_as_uint(v.w)), "r"(cluster_bar)
                  : "memory");
 }
-// 16 bytes from the shared memory of any CTA of the cluster (address from mapa).
 __device__ __forceinline__ void st_shared_cluster_v4(uint32_t cluster_addr, float4 v)
 {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");

@@ -30,9 +30,9 @@ constexpr int NORM_ROWS = 16;              // rows of a cluster
 constexpr int NORM_WARPS = 8;              // per CTA ...
 constexpr int NORM_MOST_WARPS = 16;        // ... and where eight CTAs of eight do not hold a row
 constexpr int NORM_MAX_CLUSTER = 8;        // the portable limit
-constexpr int NORM_SMEM_LIMIT = 220 * 1024;
-// behind the buffers: [2][warps] and [2][CTAs] sums of 16 rows, barriers and control words
-constexpr int NORM_FIXED_SMEM = 2 * (NORM_MOST_WARPS + NORM_MAX_CLUSTER) * NORM_ROWS * 4 + 64;
+constexpr int NORM_SMEM_LIMIT = 227 * 1024;
+// behind the buffers: two sets of sums, barriers, control word
+constexpr int norm_fixed_smem(int blocks) { return 2 * blocks * NORM_ROWS * 4 + (2 + NORM_MOST_WARPS) * 8 + 16; }
 
 struct NormParams {
     const void* x;
@@ -250,84 +250,55 @@ __device__ __forceinline__ float norm_rstd(const NormParams& p, float total)
     return __frsqrt_rn(__fadd_rn(__fmul_rn(total, p.inv_K), p.eps));
 }
 
-// Rows that a cluster holds.  grid = a multiple of the cluster size, 32 threads per block of a CTA's share.
+// Rows that a cluster holds.  grid = a multiple of the cluster size, 32 threads per block of a CTA's share.  x_map, r_map: [rows, K] in boxes of
+// 16 rows x 128 columns, zeros behind the last row (r_map is not looked at without R).
 template <class X, class R>
 __global__ void __launch_bounds__(32 * NORM_MOST_WARPS, 1)
-rmsnorm_quantize_kernel(const NormParams p)
+rmsnorm_quantize_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap r_map, const NormParams p)
 {
     constexpr bool ADD = !std::is_void<R>::value;
     using RT = typename std::conditional<ADD, R, float>::type;
-    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int X_BYTES = NORM_ROWS * 128 * static_cast<int>(sizeof(X)), R_BYTES = ADD ? NORM_ROWS * 128 * static_cast<int>(sizeof(RT)) : 0;
+    extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, C = p.cluster;
     const int rank = C > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
-    const int width = warps * 128, KB = p.K / 128, kb = rank * warps + warp;
-    const int cols = min(warps, KB - rank * warps) * 128;              // of this CTA's share, at least one block
-    uint8_t* xs = smem;
-    uint8_t* rs = xs + NORM_ROWS * width * sizeof(X);
-    float* warp_sums = reinterpret_cast<float*>(rs + (ADD ? NORM_ROWS * width * sizeof(RT) : 0));       // [2][warps][16]
-    float* cta_sums = warp_sums + 2 * NORM_MOST_WARPS * NORM_ROWS;                                      // [2][CTAs][16]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(cta_sums + 2 * NORM_MAX_CLUSTER * NORM_ROWS);          // rows, sums even, sums odd
-    const uint32_t rows_bar = ptx::smem_u32(bars), sums_bar = rows_bar + 8;
-    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(bars + 3);
+    const int KB = p.K / 128, kb = rank * warps + warp;
+    const bool mine = kb < KB;                                         // of every CTA's warps the first has a block at least
+    uint8_t* const xs = smem + warp * X_BYTES;
+    uint8_t* const rs = smem + warps * X_BYTES + warp * R_BYTES;
+    float* const sums = reinterpret_cast<float*>(smem + warps * (X_BYTES + R_BYTES));                   // [2][KB][16]
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(sums + 2 * KB * NORM_ROWS);                      // sums even, sums odd, rows of each warp
+    const uint32_t sums_bar = ptx::smem_u32(bars), rows_bar = sums_bar + 16u + 8u * static_cast<uint32_t>(warp);
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(bars + 2 + warps);
 
     // the groups of 16 rows that this cluster does, one after the other
     const int groups = p.M / NORM_ROWS, clusters = static_cast<int>(gridDim.x) / C, id = static_cast<int>(blockIdx.x) / C;
     const int g0 = static_cast<int>(static_cast<long long>(groups) * id / clusters);
     const int g1 = static_cast<int>(static_cast<long long>(groups) * (id + 1) / clusters);
-    // 16 rows of x and of r, a copy per row; every warp issues its share (a copy holds the issuing warp for 80 cycles: all 32 in one warp
-    // took a third of a round), thread 0 says how many bytes there will be.
+    // this warp's block of 16 rows, of x and of r
     auto request = [&](int g) {
-        const int rows = min(NORM_ROWS, p.rows - g * NORM_ROWS);
-        if (threadIdx.x == 0) ptx::mbar_arrive_expect_tx(rows_bar, static_cast<uint32_t>(rows * cols * (sizeof(X) + (ADD ? sizeof(RT) : 0))));
-        const int copy = warp + lane * warps, i = copy & 15;           // copies 0-15: x, 16-31: r
-        if (copy < (ADD ? 32 : 16) && i < rows) {
-            const long long row = g * NORM_ROWS + i, col = rank * width;
-            if (copy < 16)
-                ptx::bulk_load(ptx::smem_u32(xs) + i * width * static_cast<int>(sizeof(X)), static_cast<const X*>(p.x) + row * p.ldx + col,
-                               static_cast<uint32_t>(cols * sizeof(X)), rows_bar);
-            else
-                ptx::bulk_load(ptx::smem_u32(rs) + i * width * static_cast<int>(sizeof(RT)), static_cast<const RT*>(p.r) + row * p.ldr + col,
-                               static_cast<uint32_t>(cols * sizeof(RT)), rows_bar);
+        if (ptx::elect_one()) {
+            ptx::mbar_arrive_expect_tx(rows_bar, X_BYTES + R_BYTES);
+            ptx::tma_load_2d(ptx::smem_u32(xs), &x_map, kb * 128, g * NORM_ROWS, rows_bar);
+            if (ADD) ptx::tma_load_2d(ptx::smem_u32(rs), &r_map, kb * 128, g * NORM_ROWS, rows_bar);
         }
         __syncwarp();
-        if (rows < NORM_ROWS) {                      // the last 16 rows: zeros behind the last, by warp 0 before its own sums
-            if (warp == 0) {
-                for (uint32_t b = static_cast<uint32_t>(rows * width) * sizeof(X) + lane * 16; b < NORM_ROWS * width * sizeof(X); b += 512)
-                    *reinterpret_cast<uint4*>(xs + b) = make_uint4(0u, 0u, 0u, 0u);
-                if (ADD)
-                    for (uint32_t b = static_cast<uint32_t>(rows * width) * sizeof(RT) + lane * 16; b < NORM_ROWS * width * sizeof(RT); b += 512)
-                        *reinterpret_cast<uint4*>(rs + b) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            __syncthreads();
-        }
     };
     if (threadIdx.x == 0) {
-        ptx::mbar_init(rows_bar, 1);
-        ptx::mbar_init(sums_bar, 1);
-        ptx::mbar_init(sums_bar + 8, 1);
+        for (int i = 0; i < 2 + warps; ++i) ptx::mbar_init(sums_bar + 8u * static_cast<uint32_t>(i), 1);
         *abort_flag = 0u;
         ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&x_map);
+        if (ADD) ptx::prefetch_tensormap(&r_map);
     }
     __syncthreads();
     if (C > 1) ptx::cluster_arrive();                // waited for before anything is sent to a peer: its barriers exist
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    request(g0);                                     // clusters <= groups
+    if (mine) request(g0);                           // clusters <= groups
     if (C > 1) ptx::cluster_wait();
 
-    auto cta_sum = [&](const float* ws, int row) {
-        float sum = 0.0f;
-        for (int j0 = 0; j0 < warps; j0 += NORM_WARPS) {
-            float v[NORM_WARPS];
-#pragma unroll
-            for (int j = 0; j < NORM_WARPS; ++j) v[j] = j0 + j < warps ? ws[(j0 + j) * NORM_ROWS + row] : 0.0f;
-#pragma unroll
-            for (int j = 0; j < NORM_WARPS; ++j) sum += v[j];
-        }
-        return sum;
-    };
-    const bool mine = kb < KB;
-    const int k = kb * 128 + lane * 4, col = warp * 128 + lane * 4;
+    const int k = kb * 128 + lane * 4;
     f32x2 w[2] = {0ull, 0ull};
     if (mine) norm_weights(p, k, w);
     bool ok = true;
@@ -337,72 +308,72 @@ rmsnorm_quantize_kernel(const NormParams p)
     uint8_t* const dst = p.out + static_cast<size_t>(k) * p.M;
     uint32_t held[4][4];
     const uint32_t start = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(dst) >> 4), long_by = static_cast<uint32_t>(groups);
-    for (int g = g0; g < g1; ++g, ++n) {
+    for (int g = mine ? g0 : g1; g < g1; ++g, ++n) {
         const int r0 = g * NORM_ROWS;
-        const uint32_t odd = n & 1u;
-        ok = ok && wait_bounded(rows_bar, odd, abort_flag, p.status, DS_TIMEOUT_STAGE_FULL);
-        f32x2 t[16][2];
-        float part[16];
-        if (mine) norm_read_shared<X, R>(xs, rs, width, col, t);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) part[i] = mine ? sum_of_squares(t[i][0], t[i][1]) : 0.0f;
-        const float sum = sum_16_rows(part, lane);
-        float* ws = warp_sums + odd * NORM_MOST_WARPS * NORM_ROWS;
-        if ((lane & 1) == 0) ws[warp * NORM_ROWS + (lane >> 1)] = sum;
-        // everybody has read the rows, and the sums are there.  A set of sums is written again two rounds later, which the barrier of
-        // the round between keeps apart (for the peers': a CTA sends round n + 2 after it has round n + 1 from everybody).
-        ok = __syncthreads_and(ok);
+        const uint32_t odd = n & 1u, bar = sums_bar + 8u * odd;
+        float* const row_sums = sums + odd * static_cast<uint32_t>(KB * NORM_ROWS);
+        ok = wait_bounded(rows_bar, odd, abort_flag, p.status, DS_TIMEOUT_STAGE_FULL);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
+        f32x2 t[16][2];
+        norm_read_shared<X, R>(xs, rs, 128, lane * 4, t);
+        __syncwarp();
         if (g + 1 < g1) request(g + 1);
-        float total = 0.0f;
-        if (C > 1) {
-            const uint32_t bar = sums_bar + 8u * odd;
-            if (threadIdx.x == 0) ptx::mbar_arrive_expect_tx(bar, static_cast<uint32_t>(C * NORM_ROWS * 4));
-            for (int i = static_cast<int>(threadIdx.x); i < NORM_ROWS * C; i += static_cast<int>(blockDim.x)) {
-                const int row = i % NORM_ROWS;
-                const uint32_t peer = static_cast<uint32_t>(i / NORM_ROWS);
-                ptx::st_async_f32(ptx::mapa(ptx::smem_u32(cta_sums + (odd * NORM_MAX_CLUSTER + rank) * NORM_ROWS + row), peer), cta_sum(ws, row),
-                                  ptx::mapa(bar, peer));
-            }
-        } else {
-            total = cta_sum(ws, lane >> 1);
+        float part[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[i] = sum_of_squares(t[i][0], t[i][1]);
+        const float sum = sum_16_rows(part, lane);
+        // The block's 16 sums to every CTA, four of them from a lane.  A set of sums is written again two rounds later: whoever sends round n + 2
+        // has round n + 1 from every warp, which sent it after it had read the sums of round n.
+        {
+            const int q = lane & 3;
+            const uint32_t peer = static_cast<uint32_t>(lane >> 2);
+            float4 v;
+            v.x = __shfl_sync(0xffffffffu, sum, 8 * q);
+            v.y = __shfl_sync(0xffffffffu, sum, 8 * q + 2);
+            v.z = __shfl_sync(0xffffffffu, sum, 8 * q + 4);
+            v.w = __shfl_sync(0xffffffffu, sum, 8 * q + 6);
+            if (static_cast<int>(peer) < C)
+                ptx::st_async_v4(ptx::mapa(ptx::smem_u32(row_sums + kb * NORM_ROWS + 4 * q), peer), v, ptx::mapa(bar, peer));
+            if (threadIdx.x == 0) ptx::mbar_arrive_expect_tx(bar, static_cast<uint32_t>(KB * NORM_ROWS * 4));
+            __syncwarp();
         }
-        float amax = 0.0f;
-        if (mine) amax = norm_weigh<R>(p, r0, k, lane, w, t);
-        if (C > 1) {
-            ok = wait_bounded(sums_bar + 8u * odd, (n >> 1) & 1u, abort_flag, p.status, DS_TIMEOUT_PEER_PARTIAL);
-            ok = __all_sync(0xffffffffu, ok);
-            float v[NORM_MAX_CLUSTER];
+        const float amax = norm_weigh<R>(p, r0, k, lane, w, t);
+        ok = wait_bounded(bar, (n >> 1) & 1u, abort_flag, p.status, DS_TIMEOUT_PEER_PARTIAL);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        float total = 0.0f;                          // even blocks in even lanes, odd ones in odd lanes
+        for (int j0 = lane & 1; j0 < KB; j0 += 16) {
+            float v[8];
 #pragma unroll
-            for (int c = 0; c < NORM_MAX_CLUSTER; ++c) v[c] = c < C ? cta_sums[(odd * NORM_MAX_CLUSTER + c) * NORM_ROWS + (lane >> 1)] : 0.0f;
+            for (int j = 0; j < 8; ++j) v[j] = j0 + 2 * j < KB ? row_sums[(j0 + 2 * j) * NORM_ROWS + (lane >> 1)] : 0.0f;
 #pragma unroll
-            for (int c = 0; c < NORM_MAX_CLUSTER; ++c) total += v[c];
+            for (int j = 0; j < 8; ++j) total += v[j];
         }
-        if (mine && ok) {
-            norm_scale(norm_factor(p, r0, kb, lane, norm_rstd(p, total), amax), t);
-            // FIRST bit j: the bytes of column j are the first 16 of an aligned 32
-            auto leave = [&](auto first) {
-                constexpr int FIRST = decltype(first)::value;
+        total += __shfl_xor_sync(0xffffffffu, total, 1);
+        norm_scale(norm_factor(p, r0, kb, lane, norm_rstd(p, total), amax), t);
+        // FIRST bit j: the bytes of column j are the first 16 of an aligned 32
+        auto leave = [&](auto first) {
+            constexpr int FIRST = decltype(first)::value;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint8_t* to = dst + static_cast<size_t>(j) * p.M + r0;
-                    if ((FIRST >> j) & 1) {
-                        norm_bytes(t, j, held[j]);
-                        if (g + 1 == g1) store_16(to, held[j]);
-                    } else {
-                        uint32_t q[4];
-                        norm_bytes(t, j, q);
-                        if (g > g0) store_32(to - 16, held[j], q);
-                        else store_16(to, q);
-                    }
+            for (int j = 0; j < 4; ++j) {
+                uint8_t* to = dst + static_cast<size_t>(j) * p.M + r0;
+                if ((FIRST >> j) & 1) {
+                    norm_bytes(t, j, held[j]);
+                    if (g + 1 == g1) store_16(to, held[j]);
+                } else {
+                    uint32_t q[4];
+                    norm_bytes(t, j, q);
+                    if (g > g0) store_32(to - 16, held[j], q);
+                    else store_16(to, q);
                 }
-            };
-            const uint32_t even = (start + static_cast<uint32_t>(g)) & 1u, next = (even + long_by) & 1u;     // of columns 0, 2 and 1, 3
-            if (even == 0u && next == 0u) leave(std::integral_constant<int, 15>{});
-            else if (even != 0u && next != 0u) leave(std::integral_constant<int, 0>{});
-            else if (even == 0u) leave(std::integral_constant<int, 5>{});
-            else leave(std::integral_constant<int, 10>{});
-        }
+            }
+        };
+        const uint32_t even = (start + static_cast<uint32_t>(g)) & 1u, next = (even + long_by) & 1u;     // of columns 0, 2 and 1, 3
+        if (even == 0u && next == 0u) leave(std::integral_constant<int, 15>{});
+        else if (even != 0u && next != 0u) leave(std::integral_constant<int, 0>{});
+        else if (even == 0u) leave(std::integral_constant<int, 5>{});
+        else leave(std::integral_constant<int, 10>{});
     }
     if (!ok) {
         // giving up with copies possibly in flight: a bounded time to land

@@ -54,7 +54,7 @@ def check_sum(out, s):
     assert ((out.double() - s).abs() <= s.abs() * torch.finfo(out.dtype).eps / 2 * (1 + 2.0 ** -12) + 2.0 ** -24 * s.abs()).all()
 
 
-SHAPES = [(1, 128), (1, 7168), (3, 384), (15, 1024), (16, 1152), (17, 2304), (40, 512), (333, 896), (2049, 1664), (7, 6272), (64, 8192), (5, 8320), (18, 14336), (18, 16384), (33, 20480)]
+SHAPES = [(1, 128), (1, 7168), (3, 384), (15, 1024), (16, 1152), (17, 2304), (40, 512), (333, 896), (2049, 1664), (7, 6272), (64, 8192), (5, 8320), (18, 14336), (18, 16384), (33, 20480), (19, 13312), (50, 5504)]
 
 
 @pytest.mark.parametrize("rows,K", SHAPES)
