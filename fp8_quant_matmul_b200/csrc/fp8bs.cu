@@ -776,10 +776,15 @@ static int launch_rmsnorm(NormParams p, const DeviceInfo* dev, cudaStream_t st)
 {
     int element = sizeof(X);
     if constexpr (!std::is_void<R>::value) element += sizeof(R);
-    // As few CTAs per cluster as hold the row, and as few warps in each (K = 2304: 3 x 6 instead of 3 x 8).  Eight bytes per column
-    // (fp32 twice): six warps, whose buffers leave room for a second CTA.
+    // Many small CTAs: up to five warps in each, more where eight CTAs would not hold the row, in equal shares (K = 2304: 4 x 5).  From nine warps
+    // on only one CTA fits an SM; then sixteen.  With eight bytes per column seven, two of which fill an SM's shared memory, equal shares or not.
+    // Over 18 shapes of 16 to 8192 rows and four pairs of types this is 3 % behind the best number for each; up to eight (six) it was 5 %.
+    // bf16 with residual, 6144 x 4608: five 38.7 us, eight 45.6; bf16, 2000 x 10240: sixteen 20.1, ten 24.6; fp32 with residual, 6144 x 4608 and
+    // 8192 x 1536: seven 67.3 and 31.2, six 75.2 and 34.2.
     const int KB = p.K / 128, groups = p.M / NORM_ROWS;
-    const int warps = ceil_div(KB, std::min(ceil_div(KB, element == 8 ? 6 : NORM_WARPS), NORM_MAX_CLUSTER));
+    int warps = ceil_div(KB, std::min(ceil_div(KB, element == 8 ? 7 : 5), NORM_MAX_CLUSTER));
+    if (element == 8 && KB > 8) warps = std::max(warps, 7);
+    if (element < 8 && warps > 8) warps = std::max(warps, NORM_MOST_WARPS);
     const int cluster = std::min(ceil_div(KB, warps), NORM_MAX_CLUSTER);         // every CTA has a block at least
     const long long smem = static_cast<long long>(NORM_ROWS) * 128 * warps * element + norm_fixed_smem(cluster * warps);
     if (warps > NORM_MOST_WARPS || smem > NORM_SMEM_LIMIT)

@@ -92,13 +92,6 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm,
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(bar)
         : "memory");
 }
-// Untiled copy global -> shared of this CTA, counted in bytes on `bar`.  Both addresses and the size: multiples of 16 bytes.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar)
-{
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
-                 : "memory");
-}
 // Asynchronous copies of 16 or 8 bytes per thread; where `valid` is false zeros are written and `src` is not read.
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid)
 {

@@ -6,20 +6,19 @@
 //
 // The norm needs a whole row before the first byte can be written, and the bytes of a column of A want many rows side by side.
 // So 16 rows are spread over a cluster: a warp owns 16 rows x 128 columns, one scale block of each row, in registers (a lane four
-// consecutive columns of every row); the warps of up to eight CTAs hold the row, which is read once.  The CTAs exchange their rows'
-// sums of squares through distributed shared memory (64 bytes from each to each, counted by an mbarrier of the receiver).  All
-// that does not need the norm is done before the exchange: s * w and its largest magnitude per row and block; after it one factor
+// consecutive columns of every row); the warps of up to eight CTAs hold the row, which is read once.  A warp sends its rows' sums of squares
+// to every CTA (16 x 4 bytes each, st.async onto an mbarrier of the receiver that counts all blocks' bytes) and adds up all blocks' itself, in
+// a fixed order.  All that does not need the norm is done before: s * w and its largest magnitude per row and block; after it one factor
 // per row and block is left, 1 / rms times the scale.  The 16 rows of a lane's column are 16 neighbouring bytes of A, so the
 // quantised values leave straight from the registers, two groups of 16 rows (a 32-byte sector) at a time.
-// The clusters are persistent and their rows arrive by bulk copies: a CTA's buffer is requested anew as soon as its warps have it in
-// registers, so that the next 16 rows are on their way while these are reduced, exchanged and stored.
-// Sums are added in a fixed order (lanes, warps, CTAs).
-// Measured (CUDA graph, cold inputs, outputs of their own): 4096 x 7168 bf16 46 us with residual (206 MB: 4.5 TB/s; a copy reaches 6.4), 28
-// without (3.2 TB/s); 6144 x 4608 fp32 with residual 75 (4.9 TB/s); one row of 7168 4.7, the chain of a launch and one round.  What bounds it is the
-// chain of a round (rows arrive, sums, exchange, factors, stores) with two CTAs of eight warps per SM to overlap it: DRAM is at 48 % of its
-// peak, the schedulers issue in 41 % of the cycles.  A third CTA per SM does not fit in the registers without spills.
-// Rows that do not fit (more than 128 blocks, or 16 rows of a CTA's share above SMEM_LIMIT: from 13440 columns in fp32 with an
-// fp32 residual) are read twice.
+// The clusters are persistent and a warp's rows arrive by TMA, a box of 16 x 128 (zeros behind the last row) on an mbarrier of its own: the next
+// box is requested as soon as this one is in registers.  The warps of a CTA have nothing else to do with one another; with copies per row for the
+// CTA as a whole, two barriers and sums per CTA a round took up to 15 % longer.
+// Measured (CUDA graph, cold inputs, outputs of their own): 4096 x 7168 bf16 46 us with residual (206 MB: 4.5 TB/s; a copy reaches 6.4), 29
+// without (3.1 TB/s); 6144 x 4608 bf16 with residual 39 (5.1), fp32 with residual 68 (5.5); one row of 7168 3.5, with residual 4.1, the chain of a
+// launch and one round.  What bounds it: in bf16 the instructions of a round and the waits between them, 16 warps per SM at most
+// with 128 registers each; in fp32 nearly the memory.
+// Rows that do not fit (more than 16384 columns; in fp32 with an fp32 residual more than 13312) are read twice.
 #pragma once
 #include "quantize.cuh"
 #include <type_traits>
@@ -27,8 +26,8 @@
 namespace fp8bs {
 
 constexpr int NORM_ROWS = 16;              // rows of a cluster
-constexpr int NORM_WARPS = 8;              // per CTA ...
-constexpr int NORM_MOST_WARPS = 16;        // ... and where eight CTAs of eight do not hold a row
+constexpr int NORM_WARPS = 8;              // per CTA of the kernel for long rows
+constexpr int NORM_MOST_WARPS = 16;        // of the other
 constexpr int NORM_MAX_CLUSTER = 8;        // the portable limit
 constexpr int NORM_SMEM_LIMIT = 227 * 1024;
 // behind the buffers: two sets of sums, barriers, control word
