@@ -316,12 +316,13 @@ rmsnorm_quantize_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_
         if (!ok) break;
         f32x2 t[16][2];
         norm_read_shared<X, R>(xs, rs, 128, lane * 4, t);
-        __syncwarp();
-        if (g + 1 < g1) request(g + 1);
         float part[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) part[i] = sum_of_squares(t[i][0], t[i][1]);
         const float sum = sum_16_rows(part, lane);
+        // The box may be filled again once its values are in registers, which nothing says but an instruction that needs them: a load may still wait
+        // for its turn when a copy that was issued after it arrives.  A sum of squares is never -0, so the vote is always for it.
+        if (__any_sync(0xffffffffu, __float_as_uint(sum) != 0x80000000u) && g + 1 < g1) request(g + 1);
         // The block's 16 sums to every CTA, four of them from a lane.  A set of sums is written again two rounds later: whoever sends round n + 2
         // has round n + 1 from every warp, which sent it after it had read the sums of round n.
         {

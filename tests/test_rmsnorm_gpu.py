@@ -243,3 +243,18 @@ def test_x_is_its_own_residual(K):
     b = f.rmsnorm_quantize(x, w, residual=x, residual_out=x)             # all three one tensor
     assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(a, b))
     check_sum(x, s)
+
+
+@pytest.mark.parametrize("xt,rt", [(F32, None), (BF16, None), (F32, F32), (BF16, BF16)], ids=lambda t: str(t).replace("torch.", ""))
+@pytest.mark.parametrize("K", [384, 2048, 4736])
+def test_many_rounds_give_the_same_bits(K, xt, rt):
+    """Many groups of rows per cluster, inputs that stay in L2: a box must not be filled again before its rows are in registers."""
+    rows = 8000 * 2048 // max(K, 2048)
+    x, w, r = make(rows, K, xt, rt, xt, seed=K + 1)
+    values, inv, s = want(x, w, r, 1e-6, 448.0)
+    first = f.rmsnorm_quantize(x, w, residual=r)
+    check(first[0], first[1], values, inv)
+    for _ in range(12):
+        again = f.rmsnorm_quantize(x, w, residual=r)
+        assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(first, again))
+    f.last_device_status()
