@@ -173,7 +173,28 @@ __device__ __forceinline__ void norm_weights(const NormParams& p, int k, f32x2 (
     }
 }
 
-// s -> r_out (`rows` of the 16); s = s * w; returns the largest |s * w| of the block in row lane / 2.
+// Which of the 16 rows a lane answers for once the sums are in (lanes that differ in bit 2: the same one), and the first lane that does.
+__device__ __forceinline__ int row_of(int lane) { return 4 * (lane & 3) + (lane >> 3); }
+__device__ constexpr int lane_of(int row) { return (row >> 2) | ((row & 3) << 3); }
+
+// 1 / x and 1 / sqrt(x): the hardware's approximation (2^-22) and a step of Newton's method, off by 2^-24 and 1.5 times that.  Without the branches of
+// the exactly rounded forms, which were a twelfth of a round.  Where the approximation is 0 or infinite the step gives NaN, and it stays.
+__device__ __forceinline__ float reciprocal(float x)
+{
+    float y;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    const float e = __fmaf_rn(-x, y, 1.0f);
+    return fabsf(e) < 1.0f ? __fmaf_rn(y, e, y) : y;
+}
+__device__ __forceinline__ float reciprocal_root(float x)
+{
+    float y;
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    const float e = __fmaf_rn(-__fmul_rn(x, y), y, 1.0f);
+    return fabsf(e) < 1.0f ? __fmaf_rn(__fmul_rn(0.5f, y), e, y) : y;
+}
+
+// s -> r_out (`rows` of the 16); s = s * w; returns the largest |s * w| of the block in row row_of(lane).
 template <class R>
 __device__ __forceinline__ float norm_weigh(const NormParams& p, int r0, int k, int lane, const f32x2 (&w)[2], f32x2 (&s)[16][2])
 {
@@ -196,20 +217,21 @@ __device__ __forceinline__ float norm_weigh(const NormParams& p, int r0, int k, 
         s[i][1] = mul_f32x2(s[i][1], w[1]);
         const float m = warp_absmax_nan(max_nan(max_nan(fabsf(f32x2_lo(s[i][0])), fabsf(f32x2_hi(s[i][0]))),
                                                 max_nan(fabsf(f32x2_lo(s[i][1])), fabsf(f32x2_hi(s[i][1])))));
-        if ((lane >> 1) == i) mine = m;
+        if (row_of(lane) == i) mine = m;
     }
     return mine;
 }
 
-// What t = s * w is multiplied with in row lane / 2 of a 16 x 128 block before it is rounded to 8 bits; stores the inverse scale.
+// What t = s * w is multiplied with in row row_of(lane) of a 16 x 128 block before it is rounded to 8 bits; stores the inverse scale.
 // rstd, amax: 1 / rms and the largest |t| of that row.
 __device__ __forceinline__ float norm_factor(const NormParams& p, int r0, int kb, int lane, float rstd, float amax)
 {
     // the rows behind the last are zeros whatever eps is
-    const float rs = r0 + (lane >> 1) < p.rows ? rstd : 0.0f;
+    const int row = row_of(lane);
+    const float rs = r0 + row < p.rows ? rstd : 0.0f;
     const float m = max_nan(__fmul_rn(amax, rs), 1e-12f);
-    const float sc = __fmul_rn(__frcp_rn(m), p.fp8_max);                             // as in quantize.cuh
-    if ((lane & 1) == 0) p.scale_out[static_cast<size_t>(kb) * p.M + r0 + (lane >> 1)] = __frcp_rn(sc);
+    const float sc = __fmul_rn(reciprocal(m), p.fp8_max);                            // as in quantize.cuh
+    if ((lane & 4) == 0) p.scale_out[static_cast<size_t>(kb) * p.M + r0 + row] = reciprocal(sc);
     // No product may round to more than fp8_max: the factor is five roundings off at most, and eight are taken off where the
     // largest product shows one.
     const float f = __fmul_rn(rs, sc);
@@ -220,7 +242,7 @@ __device__ __forceinline__ void norm_scale(float factor, f32x2 (&t)[16][2])
 {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const float f = __shfl_sync(0xffffffffu, factor, 2 * i);
+        const float f = __shfl_sync(0xffffffffu, factor, lane_of(i));
         t[i][0] = mul_f32x2(t[i][0], pack_f32x2(f, f));
         t[i][1] = mul_f32x2(t[i][1], pack_f32x2(f, f));
     }
@@ -246,7 +268,26 @@ __device__ __forceinline__ void store_32(uint8_t* dst, const uint32_t (&a)[4], c
 
 __device__ __forceinline__ float norm_rstd(const NormParams& p, float total)
 {
-    return __frsqrt_rn(__fadd_rn(__fmul_rn(total, p.inv_K), p.eps));
+    return reciprocal_root(__fadd_rn(__fmul_rn(total, p.inv_K), p.eps));
+}
+
+// The sum over all blocks of row row_of(lane); sums: [KB][16].  A lane adds up four rows of every eighth block, then the lanes theirs.
+__device__ __forceinline__ float sum_of_blocks(const float* sums, int KB, int lane)
+{
+    const float4* from = reinterpret_cast<const float4*>(sums) + (lane & 3);
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int j0 = lane >> 2; j0 < KB; j0 += 32) {
+        float4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = j0 + 8 * j < KB ? from[(j0 + 8 * j) * (NORM_ROWS / 4)] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a = make_float4(a.x + v[j].x, a.y + v[j].y, a.z + v[j].z, a.w + v[j].w);
+    }
+    const bool b4 = (lane & 16) != 0, b3 = (lane & 8) != 0;
+    const float h0 = (b4 ? a.z : a.x) + __shfl_xor_sync(0xffffffffu, b4 ? a.x : a.z, 16);
+    const float h1 = (b4 ? a.w : a.y) + __shfl_xor_sync(0xffffffffu, b4 ? a.y : a.w, 16);
+    const float one = (b3 ? h1 : h0) + __shfl_xor_sync(0xffffffffu, b3 ? h0 : h1, 8);
+    return one + __shfl_xor_sync(0xffffffffu, one, 4);
 }
 
 // Rows that a cluster holds.  grid = a multiple of the cluster size, 32 threads per block of a CTA's share.  x_map, r_map: [rows, K] in boxes of
@@ -342,15 +383,7 @@ rmsnorm_quantize_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_
         ok = wait_bounded(bar, (n >> 1) & 1u, abort_flag, p.status, DS_TIMEOUT_PEER_PARTIAL);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        float total = 0.0f;                          // even blocks in even lanes, odd ones in odd lanes
-        for (int j0 = lane & 1; j0 < KB; j0 += 16) {
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j0 + 2 * j < KB ? row_sums[(j0 + 2 * j) * NORM_ROWS + (lane >> 1)] : 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) total += v[j];
-        }
-        total += __shfl_xor_sync(0xffffffffu, total, 1);
+        const float total = sum_of_blocks(row_sums, KB, lane);
         norm_scale(norm_factor(p, r0, kb, lane, norm_rstd(p, total), amax), t);
         // FIRST bit j: the bytes of column j are the first 16 of an aligned 32
         auto leave = [&](auto first) {
@@ -422,7 +455,7 @@ rmsnorm_quantize_long_kernel(const NormParams p)
     ptx::cluster_sync();
     float total = 0.0f;
 #pragma unroll
-    for (int c = 0; c < NORM_MAX_CLUSTER; ++c) total += cta_sums[c][lane >> 1];
+    for (int c = 0; c < NORM_MAX_CLUSTER; ++c) total += cta_sums[c][row_of(lane)];
     const float rstd = norm_rstd(p, total);
     for (int kb = kb0; kb < KB; kb += STEP) {
         const int k = kb * 128 + lane * 4;
