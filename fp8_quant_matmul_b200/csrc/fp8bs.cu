@@ -777,16 +777,24 @@ static int launch_rmsnorm(NormParams p, const DeviceInfo* dev, cudaStream_t st)
     int element = sizeof(X);
     if constexpr (!std::is_void<R>::value) element += sizeof(R);
     // Many small CTAs: up to five warps in each, more where eight CTAs would not hold the row, in equal shares (K = 2304: 4 x 5).  From nine warps
-    // on only one CTA fits an SM; then sixteen.  With eight bytes per column seven, two of which fill an SM's shared memory, equal shares or not.
-    // Over 18 shapes of 16 to 8192 rows and four pairs of types this is 3 % behind the best number for each; up to eight (six) it was 5 %.
-    // bf16 with residual, 6144 x 4608: five 38.7 us, eight 45.6; bf16, 2000 x 10240: sixteen 20.1, ten 24.6; fp32 with residual, 6144 x 4608 and
-    // 8192 x 1536: seven 67.3 and 31.2, six 75.2 and 34.2.
-    const int KB = p.K / 128, groups = p.M / NORM_ROWS;
-    int warps = ceil_div(KB, std::min(ceil_div(KB, element == 8 ? 7 : 5), NORM_MAX_CLUSTER));
-    if (element == 8 && KB > 8) warps = std::max(warps, 7);
-    if (element < 8 && warps > 8) warps = std::max(warps, NORM_MOST_WARPS);
-    const int cluster = std::min(ceil_div(KB, warps), NORM_MAX_CLUSTER);         // every CTA has a block at least
-    const long long smem = static_cast<long long>(NORM_ROWS) * 128 * warps * element + norm_fixed_smem(cluster * warps);
+    // on only one CTA fits an SM; then sixteen.  With fp32 twice the rows in flight are too many for the memory before the SM is full: seven warps
+    // per SM, in two or three CTAs where the row allows (shared memory that is asked for and not used keeps others away).  Over 14 shapes
+    // of 512 to 8192 rows this is 2 to 4 % behind the best numbers for each, 6 % with fp32 beside bf16; up to eight (six) warps and as many CTAs as
+    // fit were 5 to 8 %.  bf16 with residual, 6144 x 4608: five 38.7 us, eight 45.6; bf16, 2000 x 10240: sixteen 20.1, ten 24.6; fp32 with residual,
+    // 6144 x 4608: one CTA of six 67.1, two of six 75.2; 8192 x 2048: three of two 40.2, one of seven 43.4.
+    const int KB = p.K / 128, groups = p.M / NORM_ROWS, least = ceil_div(KB, NORM_MAX_CLUSTER);
+    int warps = 5, per_sm = 0;                                                   // 0: as many as fit
+    if (element == 8) {
+        constexpr int ROOM = 7;
+        for (per_sm = 3; per_sm > 1 && ROOM / per_sm < least; --per_sm) {}
+        warps = ROOM / per_sm;
+    }
+    warps = std::max(warps, least);
+    warps = ceil_div(KB, ceil_div(KB, warps));
+    if (!per_sm && warps > 8) warps = std::max(warps, NORM_MOST_WARPS);
+    const int cluster = ceil_div(KB, warps);                                     // every CTA has a block at least
+    long long smem = static_cast<long long>(NORM_ROWS) * 128 * warps * element + norm_fixed_smem(cluster * warps);
+    if (per_sm) smem = std::max(smem, static_cast<long long>(NORM_SMEM_LIMIT / (per_sm + 1) + 1024));
     if (warps > NORM_MOST_WARPS || smem > NORM_SMEM_LIMIT)
         return launch_grid(rmsnorm_quantize_long_kernel<X, R>, dim3(static_cast<unsigned>(groups * NORM_MAX_CLUSTER), 1, 1), NORM_MAX_CLUSTER,
                            32 * NORM_WARPS, 0, st, p);
