@@ -367,7 +367,8 @@ def gemm_bias_act(A, B, a_scale, b_scale, C=None, M=None, N=None, K=None, bias=N
     """C = act(A @ B^T + bias) + residual on the current CUDA stream, in fp32 until the one rounding to bf16.
 
     A, B, a_scale, b_scale, M, N, K as in gemm().  bias: [N], fp32 or bf16.  activation: "none", "relu", "silu", "gelu" (erf) or "gelu_tanh".
-    residual: bf16 [rows, N], any row stride of whole 16 bytes; C may be the residual itself.  rows (default M): how many of the M rows
+    residual: bf16 [rows, N], any row stride of whole 16 bytes; C may be the residual itself (any other
+    overlap of the two is refused).  rows (default M): how many of the M rows
     exist in C and in the residual, e.g. 1 for one token whose A is padded to 16 rows.  splits / tile_n force a kernel.
     """
     torch = _torch()
@@ -528,7 +529,8 @@ def rmsnorm_quantize(X, weight, residual=None, eps=1e-6, fp8_max=448.0, residual
         s = X + residual;  y = s / sqrt(mean(s^2) + eps) * weight   (fp32);  then the scaling of quantize_rowwise
 
     Returns (A bytes column-major, flat; inverse scales, flat) for M = rows rounded up to a multiple of 16, the rows behind the last
-    being zeros; with a residual also s in the residual's type, in residual_out if that is given (which may be the residual, or X).
+    being zeros; with a residual also s in the residual's type, in residual_out if that is given (which may be the residual, or X; any
+    other overlap with them is refused).
     X, residual and weight: fp32 or bf16 each.  X and residual may be column slices (any row stride of whole 16 bytes).
     """
     torch = _torch()
