@@ -777,11 +777,14 @@ static int launch_rmsnorm(NormParams p, const DeviceInfo* dev, cudaStream_t st)
     int element = sizeof(X);
     if constexpr (!std::is_void<R>::value) element += sizeof(R);
     // Many small CTAs: up to five warps in each, more where eight CTAs would not hold the row, in equal shares (K = 2304: 4 x 5).  From nine warps
-    // on only one CTA fits an SM; then sixteen.  With fp32 twice the rows in flight are too many for the memory before the SM is full: seven warps
-    // per SM, in two or three CTAs where the row allows (shared memory that is asked for and not used keeps others away).  Over 14 shapes
-    // of 512 to 8192 rows this is 2 to 4 % behind the best numbers for each, 6 % with fp32 beside bf16; up to eight (six) warps and as many CTAs as
-    // fit were 5 to 8 %.  bf16 with residual, 6144 x 4608: five 38.7 us, eight 45.6; bf16, 2000 x 10240: sixteen 20.1, ten 24.6; fp32 with residual,
-    // 6144 x 4608: one CTA of six 67.1, two of six 75.2; 8192 x 2048: three of two 40.2, one of seven 43.4.
+    // on only one CTA fits an SM; then sixteen.
+    // With a residual the rows in flight get too many for the memory before the SM is full.  bf16 twice: up to eleven warps, one CTA per SM, where
+    // five are not enough, but not for the few rows of one or two rounds.  fp32 twice: seven warps per SM, in two or three CTAs where the row
+    // allows (shared memory that is asked for and not used keeps others away).
+    // Over 14 shapes of 512 to 8192 rows this is 2 to 4 % behind the best numbers for each, 6 % with fp32 beside bf16; up to eight (six) warps and
+    // as many CTAs as fit were 5 to 8 %.  bf16 with residual, 6144 x 4608: five 38.7 us, eight 45.6; 4096 x 7168: ten 44.5, seven 46.2; 16 x 7168: seven
+    // 4.2, ten 4.7.  bf16, 2000 x 10240: sixteen 20.1, ten 24.6.  fp32 with residual, 6144 x 4608: one CTA of six 67.1, two of six 75.2; 8192 x
+    // 2048: three of two 40.2, one of seven 43.4.
     const int KB = p.K / 128, groups = p.M / NORM_ROWS, least = ceil_div(KB, NORM_MAX_CLUSTER);
     int warps = 5, per_sm = 0;                                                   // 0: as many as fit
     if (element == 8) {
@@ -789,9 +792,10 @@ static int launch_rmsnorm(NormParams p, const DeviceInfo* dev, cudaStream_t st)
         for (per_sm = 3; per_sm > 1 && ROOM / per_sm < least; --per_sm) {}
         warps = ROOM / per_sm;
     }
+    if (!std::is_void<R>::value && element == 4 && least > 5 && groups > 16) warps = 11;
     warps = std::max(warps, least);
     warps = ceil_div(KB, ceil_div(KB, warps));
-    if (!per_sm && warps > 8) warps = std::max(warps, NORM_MOST_WARPS);
+    if (!per_sm && least > 8) warps = std::max(warps, NORM_MOST_WARPS);
     const int cluster = ceil_div(KB, warps);                                     // every CTA has a block at least
     long long smem = static_cast<long long>(NORM_ROWS) * 128 * warps * element + norm_fixed_smem(cluster * warps);
     if (per_sm) smem = std::max(smem, static_cast<long long>(NORM_SMEM_LIMIT / (per_sm + 1) + 1024));
