@@ -758,7 +758,7 @@ static int encode_norm_map(CUtensorMap* tm, const void* base, int rows, int K, l
 {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * sizeof(T)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(rows > 1 ? ld : K) * sizeof(T)};       // below 2^40, whatever a single row's is said to be
     const cuuint32_t box[2] = {128u, static_cast<cuuint32_t>(NORM_ROWS)};
     const cuuint32_t estr[2] = {1u, 1u};
     const CUresult r = g_encode_tiled(tm, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base), dims, strides, box,

@@ -14,7 +14,7 @@
 // The clusters are persistent and a warp's rows arrive by TMA, a box of 16 x 128 (zeros behind the last row) on an mbarrier of its own: the next
 // box is requested as soon as this one is in registers.  The warps of a CTA have nothing else to do with one another; with copies per row for the
 // CTA as a whole, two barriers and sums per CTA a round took up to 15 % longer.
-// Measured (CUDA graph, cold inputs, outputs of their own): 4096 x 7168 bf16 44 us with residual (206 MB: 4.6 TB/s; a copy reaches 6.4), 28
+// Measured (CUDA graph, cold inputs, outputs of their own): 4096 x 7168 bf16 43-44 us with residual (206 MB: 4.7 TB/s; a copy reaches 6.4), 28
 // without (3.2 TB/s); 6144 x 4608 bf16 with residual 39 (5.1), fp32 with residual 67 (5.5); one row of 7168 3.4, with residual 4.1, the chain of a
 // launch and one round.  What bounds it: in bf16 the instructions of a round and the waits between them, 16 warps per SM at most
 // with 128 registers each; in fp32 nearly the memory.

@@ -258,3 +258,14 @@ def test_many_rounds_give_the_same_bits(K, xt, rt):
         again = f.rmsnorm_quantize(x, w, residual=r)
         assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(first, again))
     f.last_device_status()
+
+
+def test_the_pitch_of_a_single_row_does_not_matter():
+    K = 640
+    x, w, r = make(1, K, BF16, F32, F32, seed=31)
+    a = f.rmsnorm_quantize(x, w, residual=r)
+    q, sc, ro = torch.empty_like(a[0]), torch.empty_like(a[1]), torch.empty_like(a[2])
+    rc = f.lib().fp8bs_rmsnorm_quantize(x.data_ptr(), 1, 1 << 50, r.data_ptr(), 0, 1 << 50, ro.data_ptr(), w.data_ptr(), 0, q.data_ptr(), sc.data_ptr(), 1, K, 1e-6, 448.0,
+                                        torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert all(torch.equal(p.view(torch.uint8), o.view(torch.uint8)) for p, o in zip(a, (q, sc, ro)))
