@@ -385,6 +385,41 @@ def test_one_matrix_in_both_places():
         close_bf16(H, h, err)
 
 
+
+def test_side_by_side_on_four_streams_the_bits_stay_the_same():
+    """The norm and every kind of fused kernel at once, so that each is held up by others at changing places."""
+    def norm(rows, K, xt, rt):
+        x = torch.randn(rows, K, device=DEV).to(xt)
+        r = None if rt is None else torch.randn(rows, K, device=DEV).to(rt)
+        w = torch.rand(K, device=DEV)
+        return lambda: f.rmsnorm_quantize(x, w, residual=r)
+
+    def gated(M, N, K, **kw):
+        args, _ = gated_operands(M, M, N, K)
+        return lambda: f.gemm_gated(*args, M=M, N=N, K=K, quantize=True, **kw)
+
+    def act(M, N, K, **kw):
+        (A, B, _, a_s, b_s, _), _ = gated_operands(M, M, N, K)
+        bias, R = torch.randn(N, device=DEV), torch.randn(M, N, device=DEV).to(BF16)
+        return lambda: (f.gemm_bias_act(A, B, a_s, b_s, M=M, N=N, K=K, bias=bias, activation="gelu", residual=R, **kw),)
+
+    jobs = [norm(2048, 2048, F32, None), norm(1000, 7168, BF16, BF16), norm(3000, 512, BF16, None), norm(777, 4608, F32, F32), norm(40, 20480, F32, BF16),
+            gated(272, 512, 1152, splits=3, tile_n=256), gated(64, 1024, 1024), gated(1040, 768, 512), act(1040, 1552, 384, tile_n=PAIR),
+            act(528, 1040, 640, tile_n=128, splits=1), act(272, 528, 1024, splits=2, tile_n=128)]
+    first = [job() for job in jobs]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    for round_of_calls in range(10):
+        outs = []
+        for i, job in enumerate(jobs * 3):
+            with torch.cuda.stream(streams[(i + round_of_calls) % 4]):
+                outs.append((i % len(jobs), job()))
+        torch.cuda.synchronize()
+        for i, out in outs:
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(first[i], out)), i
+    f.last_device_status()
+
+
 FIRST_CALLS = """
 import torch, fp8_quant_matmul_b200 as f
 K, N = 256, 256
