@@ -226,15 +226,14 @@ __device__ __forceinline__ float norm_weigh(const NormParams& p, int r0, int k, 
 // rstd, amax: 1 / rms and the largest |t| of that row.
 __device__ __forceinline__ float norm_factor(const NormParams& p, int r0, int kb, int lane, float rstd, float amax)
 {
-    // the rows behind the last are zeros whatever eps is
+    // the rows behind the last have the scale of zeros, whatever eps and the weight are, and their bytes are masked
     const int row = row_of(lane);
-    const float rs = r0 + row < p.rows ? rstd : 0.0f;
-    const float m = max_nan(__fmul_rn(amax, rs), 1e-12f);
+    const float m = r0 + row < p.rows ? max_nan(__fmul_rn(amax, rstd), 1e-12f) : 1e-12f;
     const float sc = __fmul_rn(reciprocal(m), p.fp8_max);                            // as in quantize.cuh
     if ((lane & 4) == 0) p.scale_out[static_cast<size_t>(kb) * p.M + r0 + row] = reciprocal(sc);
     // No product may round to more than fp8_max: the factor is five roundings off at most, and eight are taken off where the
     // largest product shows one.
-    const float f = __fmul_rn(rs, sc);
+    const float f = __fmul_rn(rstd, sc);
     return __fmul_rn(amax, f) > p.fp8_max ? __fmul_rn(f, 1.0f - 0x1p-21f) : f;
 }
 // t = t * factor
@@ -247,12 +246,25 @@ __device__ __forceinline__ void norm_scale(float factor, f32x2 (&t)[16][2])
         t[i][1] = mul_f32x2(t[i][1], pack_f32x2(f, f));
     }
 }
-// The bytes of column j of a lane's four, 16 rows.
-__device__ __forceinline__ void norm_bytes(const f32x2 (&t)[16][2], int j, uint32_t (&q)[4])
+// Which bytes of a column's 16 are rows that exist: those behind the last are +0, which a product with a negative weight, or one that is not
+// finite, is not.
+__device__ __forceinline__ void norm_rows_mask(int rows, uint32_t (&mask)[4])
+{
+#pragma unroll
+    for (int g = 0; g < 4; ++g) asm("shl.b32 %0, -1, %1;" : "=r"(mask[g]) : "r"(max(8 * (rows - 4 * g), 0)));      // by 32 or more: 0
+#pragma unroll
+    for (int g = 0; g < 4; ++g) mask[g] = ~mask[g];
+}
+// The bytes of column j of a lane's four, 16 rows; those that exist of the last 16 (WHOLE false).
+template <bool WHOLE>
+__device__ __forceinline__ void norm_bytes(const f32x2 (&t)[16][2], const uint32_t (&mask)[4], int j, uint32_t (&q)[4])
 {
     auto v = [&](int i) { return (j & 1) ? f32x2_hi(t[i][j >> 1]) : f32x2_lo(t[i][j >> 1]); };
 #pragma unroll
-    for (int g = 0; g < 4; ++g) q[g] = cvt_e4m3x2(v(4 * g), v(4 * g + 1)) | (cvt_e4m3x2(v(4 * g + 2), v(4 * g + 3)) << 16);
+    for (int g = 0; g < 4; ++g) {
+        q[g] = cvt_e4m3x2(v(4 * g), v(4 * g + 1)) | (cvt_e4m3x2(v(4 * g + 2), v(4 * g + 3)) << 16);
+        if constexpr (!WHOLE) q[g] &= mask[g];
+    }
 }
 
 __device__ __forceinline__ void store_16(uint8_t* dst, const uint32_t (&q)[4])
@@ -385,22 +397,30 @@ rmsnorm_quantize_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_
         if (!ok) break;
         const float total = sum_of_blocks(row_sums, KB, lane);
         norm_scale(norm_factor(p, r0, kb, lane, norm_rstd(p, total), amax), t);
-        // FIRST bit j: the bytes of column j are the first 16 of an aligned 32
-        auto leave = [&](auto first) {
+        // FIRST bit j: the bytes of column j are the first 16 of an aligned 32.  (The mask in every round, with its registers, was 4 % of 4096 x 7168 bf16
+        // without residual.)
+        auto leave_rows = [&](auto first, auto whole) {
             constexpr int FIRST = decltype(first)::value;
+            constexpr bool WHOLE = decltype(whole)::value;
+            uint32_t mask[4];
+            if constexpr (!WHOLE) norm_rows_mask(p.rows - r0, mask);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint8_t* to = dst + static_cast<size_t>(j) * p.M + r0;
                 if ((FIRST >> j) & 1) {
-                    norm_bytes(t, j, held[j]);
+                    norm_bytes<WHOLE>(t, mask, j, held[j]);
                     if (g + 1 == g1) store_16(to, held[j]);
                 } else {
                     uint32_t q[4];
-                    norm_bytes(t, j, q);
+                    norm_bytes<WHOLE>(t, mask, j, q);
                     if (g > g0) store_32(to - 16, held[j], q);
                     else store_16(to, q);
                 }
             }
+        };
+        auto leave = [&](auto first) {
+            if (p.rows - r0 >= NORM_ROWS) leave_rows(first, std::true_type{});
+            else leave_rows(first, std::false_type{});
         };
         const uint32_t even = (start + static_cast<uint32_t>(g)) & 1u, next = (even + long_by) & 1u;     // of columns 0, 2 and 1, 3
         if (even == 0u && next == 0u) leave(std::integral_constant<int, 15>{});
@@ -464,12 +484,19 @@ rmsnorm_quantize_long_kernel(const NormParams p)
         norm_weights(p, k, w);
         const float amax = norm_weigh<R>(p, r0, k, lane, w, t);
         norm_scale(norm_factor(p, r0, kb, lane, rstd, amax), t);
+        auto leave = [&](auto whole) {
+            constexpr bool WHOLE = decltype(whole)::value;
+            uint32_t mask[4];
+            if constexpr (!WHOLE) norm_rows_mask(p.rows - r0, mask);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t q[4];
-            norm_bytes(t, j, q);
-            store_16(p.out + static_cast<size_t>(k + j) * p.M + r0, q);
-        }
+            for (int j = 0; j < 4; ++j) {
+                uint32_t q[4];
+                norm_bytes<WHOLE>(t, mask, j, q);
+                store_16(p.out + static_cast<size_t>(k + j) * p.M + r0, q);
+            }
+        };
+        if (p.rows - r0 >= NORM_ROWS) leave(std::true_type{});
+        else leave(std::false_type{});
     }
 }
 

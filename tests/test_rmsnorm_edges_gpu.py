@@ -1,0 +1,55 @@
+"""rmsnorm_quantize where its promises are narrow: the rows behind the last, and the scales counted rounding by rounding.
+
+The roundings of an inverse scale, U = 2^-24 each, before any run.  The sum of squares of a row: a lane's four columns 3 (two products, of which one
+is part of a multiply-add, and two additions), the 32 lanes 5, then the row's blocks: rows that a cluster holds, every eighth block to a lane, 3 more
+between the lanes; longer rows, a warp's blocks one after the other, 8 warps, 8 CTAs.  All terms are positive, so the count bounds the
+relative error.  The mean adds 2 (1 / K is rounded too), eps 1; the root halves it all and adds 1.5 of its own; the rounding of s = x + r counts once under the root
+and once as the value.  Then the product with the weight, with 1 / rms, the reciprocal, the product with fp8_max and the second reciprocal: 5.
+A reciprocal is a Newton step on the hardware's approximation (2^-22): its error is squared away, the last multiply-add rounds once.  The root's step has
+a rounded product in it, half of whose error stays."""
+import pytest
+
+import fp8_quant_matmul_b200 as f
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+BF16, F32 = torch.bfloat16, torch.float32
+DEV = "cuda"
+U = 2.0 ** -24
+
+
+def scale_roundings(K, long_rows, with_residual):
+    blocks = K // 128
+    if long_rows:
+        squares = 3 + 5 + (blocks + 63) // 64 + 8 + 8
+    else:
+        squares = 3 + 5 + (blocks + 7) // 8 - 1 + 3
+    return 0.5 * (squares + 3) + 1.5 + 5 + (2 if with_residual else 0)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 16, 17, 31])
+@pytest.mark.parametrize("K", [256, 1152, 20480])
+@pytest.mark.parametrize("xt,rt", [(BF16, None), (F32, None), (BF16, BF16), (F32, F32), (BF16, F32)], ids=lambda t: str(t).replace("torch.", ""))
+def test_rows_behind_the_last_are_zero_bytes_whatever_the_weights(rows, K, xt, rt):
+    g = torch.Generator().manual_seed(rows + K)
+    x = torch.randn(rows, K, generator=g).to(xt).to(DEV)
+    r = None if rt is None else torch.randn(rows, K, generator=g).to(rt).to(DEV)
+    M = (rows + 15) // 16 * 16
+    for special in ((), (float("nan"),), (float("inf"), float("-inf"))):
+        w = torch.randn(K, generator=g)
+        assert (w < 0).any()
+        for i, v in enumerate(special):
+            w[3 + 130 * i] = v
+        q, sc = f.rmsnorm_quantize(x, w.to(DEV), residual=r)[:2]
+        assert (q.view(K, M)[:, rows:] == 0).all()
+        # 1 / (fp8_max / 1e-12): two reciprocals, a product and the constant's own rounding
+        behind = sc.view(K // 128, M)[:, rows:].double()
+        assert ((behind - 1e-12 / 448.0).abs() <= 4 * U * 1e-12 / 448.0).all()
+        if not special:
+            values = (x.double() + (0 if r is None else r.double()))
+            values = values / torch.sqrt((values * values).mean(1, keepdim=True) + 1e-6) * w.to(DEV).double()
+            inv = values.view(rows, K // 128, 128).abs().amax(2) / 448.0
+            tol = scale_roundings(K, K > 16384, r is not None) * U
+            assert ((sc.view(K // 128, M)[:, :rows].t().double() - inv).abs() <= tol * inv).all()
+    f.last_device_status()
