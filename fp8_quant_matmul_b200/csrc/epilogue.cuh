@@ -6,8 +6,9 @@
 // number.  4096 x 7168 x 512 with bias on pair tiles: 23 us without activation, relu 24, silu 37, gelu_tanh 38, gelu 44; a copy of silu without
 // any exponential or reciprocal took 2 us less, and steps interleaved over two, four or eight pairs of values are no faster.  Two values
 // share one reciprocal (1 / d0 = d1 / (d0 d1)).
-// Errors (2^-22 of the exponential and of the reciprocal, and the argument's rounding) are below 1 % of a bf16 step where the result is not itself
-// negligible, and an output in 8 bits has its scale from the largest elements, where the exponential is next to nothing.
+// Errors (2^-22 of the exponential and of the reciprocal, the rounding of the argument): silu below 2^-17 of the result down to -40, gelu_tanh 2^-16 down to
+// -7.4, less than 1 % of a bf16 step; below that they stay at -2e-16 and -2e-17 while the formulas go on to 0.  gelu: 7.5e-8 |x| of its formula and
+// 2^-19 of erfc's share of the result.  An output in 8 bits has its scale from the largest elements, where the exponential is next to nothing.
 // (In packed fp32 instructions the activations were no faster and the K loop of the pair kernel, which shares their registers, 17 %
 // slower, whichever was chosen at run time.)
 #pragma once
@@ -97,8 +98,10 @@ __device__ __forceinline__ unsigned long long gelu_tanh_2(unsigned long long x)
     return logistic_times_2(x0, x1, t0 * fmaf(t0 * t0, B, A), t1 * fmaf(t1 * t1, B, A));
 }
 // gelu: x (1 + erf(x / sqrt 2)) / 2 = max(x, 0) - |x| erfc(|x| / sqrt 2) / 2 with erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), t = 1 / (1 + p z): formula
-// 7.1.26 of Abramowitz and Stegun, off by 1.5e-7 at most, that is 7.5e-8 |x| here; and the tail below 0 has no cancellation.  (CUDA's
-// erff in this place cost the K loop of the pair kernel 15 spilled registers.)
+// 7.1.26 of Abramowitz and Stegun, off by 1.5e-7 at most, that is 7.5e-8 |x| here, about what 1 + erf loses in fp32 as soon as erf is near -1.  Relative
+// to the result the formula is off by 5e-5 at -3, 5e-4 at -4 (result -1.3e-4), 1.6e-3 at -5 and 3.6e-3 at -6 (-6e-9), where half a bf16 step is 2e-3 to
+// 3.9e-3: below -3.5 the last bit of a bf16 result is not always the formula's.  (A sixth term and coefficients fitted for the tail give
+// 3e-5 everywhere, but 48.4 -> 50.7 us on 4096 x 7168 x 512.  CUDA's erff in this place cost the K loop of the pair kernel 15 spilled registers.)
 __device__ __forceinline__ unsigned long long gelu_2(unsigned long long x)
 {
     const float x0 = f32x2_lo(x), x1 = f32x2_hi(x);

@@ -139,7 +139,8 @@ int fp8bs_gemm_ex(const void* A, const void* B, const float* a_scale, const floa
  * what fp8bs_gemm rounds.  M, N, K and the operands as there; of the M rows the first `rows` (1..M) exist in C and in the residual:
  * nothing is written behind them, so that a call for one token (A padded to 16 rows) has a C of one row.
  *   bias        [N], bf16 (bias_is_bf16 != 0) or fp32, 16-byte aligned; NULL: none
- *   activation  FP8BS_ACT_*
+ *   activation  FP8BS_ACT_*.  Evaluated in fp32: silu to 2^-17 of its value (at -2e-16 below arguments of -40), gelu_tanh to 2^-16 (at -2e-17 below
+ *               -7.4), gelu to 7.5e-8 of its argument, as 1 + erf in fp32 would be
  *   residual    [rows, N] bf16 with a row pitch of ld_residual elements (>= N, a multiple of 8), 16-byte aligned; NULL: none.  It may be
  *               C itself (ld_residual = N); any other overlap with C is refused.
  *   splits      0 = let the library choose; 1..8 = K cut over a cluster of that many CTAs
