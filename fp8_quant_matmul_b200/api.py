@@ -341,16 +341,18 @@ def _check_fused(index, M, N, K, rows, activation, A, a_scale, weights):
         raise ValueError("M, N, K are required (operands are flat column-major buffers)")
     if not 1 <= rows <= M:
         raise ValueError("rows has to be in 1..M")
+    torch = _torch()
+    byte, fp8, f32 = torch.uint8, torch.float8_e4m3fn, torch.float32       # another 1-byte type would be read as e4m3fn all the same
     blocks = K // 128
-    good = (A.numel() >= M * K and A.element_size() == 1 and A.is_contiguous() and a_scale.get_device() == index
-            and a_scale.numel() >= M * blocks and a_scale.element_size() == 4 and a_scale.is_contiguous())
+    good = (A.numel() >= M * K and (A.dtype is byte or A.dtype is fp8) and A.is_contiguous() and a_scale.get_device() == index
+            and a_scale.numel() >= M * blocks and a_scale.dtype is f32 and a_scale.is_contiguous())
     n, n_scale = N * K, (N + 127) // 128 * blocks
     for B, scale in weights:
-        good = (good and B.get_device() == index and B.numel() >= n and B.element_size() == 1 and B.is_contiguous()
-                and scale.get_device() == index and scale.numel() >= n_scale and scale.element_size() == 4 and scale.is_contiguous())
+        good = (good and B.get_device() == index and B.numel() >= n and (B.dtype is byte or B.dtype is fp8) and B.is_contiguous()
+                and scale.get_device() == index and scale.numel() >= n_scale and scale.dtype is f32 and scale.is_contiguous())
     if not good:
-        raise ValueError("operands have to be contiguous tensors on A's device: 1-byte elements of M*K and N*K, fp32 scales of M*K/128 and "
-                         "ceil(N/128)*K/128")
+        raise ValueError("operands have to be contiguous tensors on A's device: uint8 or float8_e4m3fn of M*K and N*K elements, fp32 scales of M*K/128 "
+                         "and ceil(N/128)*K/128")
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError("activation has to be one of " + ", ".join(ACTIVATIONS))
