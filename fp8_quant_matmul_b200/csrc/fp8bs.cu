@@ -991,7 +991,8 @@ static int fused_impl(const void* A, const void* B, const void* B2, const float*
     if ((rc = encode_operand_map(&tm.B, B, N, K))) return rc;
     if (gated && (rc = encode_operand_map(&tm.C.m[MAP_UP], B2, N, K))) return rc;
     if (cfg.mode != 5 && (rc = fp8 ? encode_operand_map(&tm.C.m[0], out, M, N) : encode_c_map(&tm.C.m[0], out, rows, N, N))) return rc;
-    if (residual && cfg.mode == 0 && (rc = encode_c_map(&tm.C.m[MAP_RESIDUAL], const_cast<void*>(residual), rows, N, ldr))) return rc;
+    // (the pitch of a single row is not used, whatever it is said to be; a map takes one below 2^40 bytes)
+    if (residual && cfg.mode == 0 && (rc = encode_c_map(&tm.C.m[MAP_RESIDUAL], const_cast<void*>(residual), rows, N, rows > 1 ? ldr : N))) return rc;
     GemmParams p = gemm_params(cfg, gated ? 128 : cfg.tile_n, a_scale, b_scale, out, M, N, K, 0, N, dev->status_ptr, st);
     p.rows = rows;
     Epilogue e{};
