@@ -724,7 +724,8 @@ static int launch_gated(const DeviceInfo* dev, const Config& c, const TensorMaps
     return c.cg == 2 ? launch_fused<256, 2, 0, EPI>(dev, tm, p, st, e) : launch_fused<256, 1, 0, EPI>(dev, tm, p, st, e);
 }
 
-// How many clusters of `cluster` CTAs with `warps` warps of the norm kernel run at once: asked once per device, type and shape.
+// How many clusters of `cluster` CTAs with `warps` warps of the norm kernel run at once: asked once per device, type and shape (the choice below gives a
+// shape of a type always the same shared memory).
 template <class X, class R>
 static int norm_clusters(int device, int cluster, int warps, int smem, int* out)
 {
@@ -777,34 +778,48 @@ static int launch_rmsnorm(NormParams p, const DeviceInfo* dev, cudaStream_t st)
     int element = sizeof(X);
     if constexpr (!std::is_void<R>::value) element += sizeof(R);
     // Many small CTAs: up to five warps in each, more where eight CTAs would not hold the row, in equal shares (K = 2304: 4 x 5).  From nine warps
-    // on only one CTA fits an SM; then sixteen.
-    // With a residual the rows in flight get too many for the memory before the SM is full.  bf16 twice: up to eleven warps, one CTA per SM, where
-    // five are not enough, but not for the few rows of one or two rounds.  fp32 twice: seven warps per SM, in two or three CTAs where the row
-    // allows (shared memory that is asked for and not used keeps others away).
-    // Over 14 shapes of 512 to 8192 rows this is 2 to 4 % behind the best numbers for each, 6 % with fp32 beside bf16; up to eight (six) warps and
-    // as many CTAs as fit were 5 to 8 %.  bf16 with residual, 6144 x 4608: five 38.7 us, eight 45.6; 4096 x 7168: ten 44.5, seven 46.2; 16 x 7168: seven
-    // 4.2, ten 4.7.  bf16, 2000 x 10240: sixteen 20.1, ten 24.6.  fp32 with residual, 6144 x 4608: one CTA of six 67.1, two of six 75.2; 8192 x
-    // 2048: three of two 40.2, one of seven 43.4.
-    const int KB = p.K / 128, groups = p.M / NORM_ROWS, least = ceil_div(KB, NORM_MAX_CLUSTER);
-    int warps = 5, per_sm = 0;                                                   // 0: as many as fit
+    // on only one CTA fits an SM.
+    // With a residual the rows in flight get too many for the memory before the SM is full.  fp32 twice: seven warps per SM, in two or three CTAs where the
+    // row allows (shared memory that is asked for and not used keeps others away).  fp32 with residual, 6144 x 4608: one CTA of six 67.1 us, two of
+    // six 75.2; 8192 x 2048: three of two 40.2, one of seven 43.4.  bf16 with residual, 6144 x 4608: five warps 38.7, eight 45.6.
+    const int KB = p.K / 128, groups = p.M / NORM_ROWS, least = ceil_div(KB, NORM_MAX_CLUSTER), device = static_cast<int>(dev - g_dev);
+    auto equal_shares = [&](int warps) { return ceil_div(KB, ceil_div(KB, warps)); };
+    auto smem_of = [&](int warps) {
+        return static_cast<long long>(NORM_ROWS) * 128 * warps * element + norm_fixed_smem(ceil_div(KB, warps) * warps);
+    };
+    int warps = 5, per_sm = 0, rc = FP8BS_OK, most = 0;                          // per_sm 0: as many as fit
     if (element == 8) {
         constexpr int ROOM = 7;
         for (per_sm = 3; per_sm > 1 && ROOM / per_sm < least; --per_sm) {}
         warps = ROOM / per_sm;
     }
-    if (!std::is_void<R>::value && element == 4 && least > 5 && groups > 16) warps = 11;
-    warps = std::max(warps, least);
-    warps = ceil_div(KB, ceil_div(KB, warps));
-    if (!per_sm && least > 8) warps = std::max(warps, NORM_MOST_WARPS);
+    warps = equal_shares(std::max(warps, least));
+    if (per_sm == 0 && least <= NORM_MOST_WARPS && (least > 8 || (!std::is_void<R>::value && element == 4 && least > 5))) {
+        // Rows over 8192 columns, and over 5120 of bf16 with a bf16 residual: the shape of eight to four CTAs whose clusters do all groups in the
+        // fewest rounds, where that is one or two; of equals the one with the fewest warps on an SM.  Else up to eleven warps, one CTA per SM; over 8192
+        // columns six CTAs, over 12288 eight (few clusters of seven find room).
+        // bf16 with residual, us: 16 x 7168 7 warps x 8 CTAs 3.8, 10 x 6 4.2; 256 rows 10 x 6 6.4, 7 x 8 6.9; 368 rows 12 x 5 7.4, 7 x 8 7.6, 10 x 6 9.3; 4096
+        // rows 10 x 6 43.7, 7 x 8 46.1; 64 x 9216 9 x 8 5.2, 15 x 5 6.2; 1400 x 9216 12 x 6 18.6, 9 x 8 21.7, 15 x 5 22.5.
+        int rounds = 3, on_sm = 0;
+        warps = least <= 8 ? equal_shares(11) : ceil_div(KB, 6) <= NORM_MOST_WARPS ? ceil_div(KB, 6) : least;
+        for (int c = NORM_MAX_CLUSTER; c >= 4 && ceil_div(KB, c) <= NORM_MOST_WARPS; --c) {
+            const int w = ceil_div(KB, c), cluster = ceil_div(KB, w), alone = dev->model.max_clusters[cluster];
+            if ((rc = norm_clusters<X, R>(device, cluster, w, static_cast<int>(smem_of(w)), &most))) return rc;
+            const int r = ceil_div(groups, most), o = groups > alone && most >= 2 * alone ? 2 * w : w;
+            if (r < rounds || (r == rounds && r < 3 && o < on_sm)) {
+                rounds = r;
+                on_sm = o;
+                warps = w;
+            }
+        }
+    }
     const int cluster = ceil_div(KB, warps);                                     // every CTA has a block at least
-    long long smem = static_cast<long long>(NORM_ROWS) * 128 * warps * element + norm_fixed_smem(cluster * warps);
+    long long smem = smem_of(warps);
     if (per_sm) smem = std::max(smem, static_cast<long long>(NORM_SMEM_LIMIT / (per_sm + 1) + 1024));
     if (warps > NORM_MOST_WARPS || smem > NORM_SMEM_LIMIT)
         return launch_grid(rmsnorm_quantize_long_kernel<X, R>, dim3(static_cast<unsigned>(groups * NORM_MAX_CLUSTER), 1, 1), NORM_MAX_CLUSTER,
                            32 * NORM_WARPS, 0, st, p);
-    int most = 0;
-    int rc = norm_clusters<X, R>(static_cast<int>(dev - g_dev), cluster, warps, static_cast<int>(smem), &most);
-    if (rc) return rc;
+    if ((rc = norm_clusters<X, R>(device, cluster, warps, static_cast<int>(smem), &most))) return rc;
     CUtensorMap x_map{}, r_map{};
     if ((rc = encode_norm_map<X>(&x_map, p.x, p.rows, p.K, p.ldx))) return rc;
     if constexpr (!std::is_void<R>::value)

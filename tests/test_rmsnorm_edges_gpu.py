@@ -53,3 +53,27 @@ def test_rows_behind_the_last_are_zero_bytes_whatever_the_weights(rows, K, xt, r
             tol = scale_roundings(K, K > 16384, r is not None) * U
             assert ((sc.view(K // 128, M)[:, :rows].t().double() - inv).abs() <= tol * inv).all()
     f.last_device_status()
+
+
+@pytest.mark.parametrize("K", [5248, 6144, 7168, 8192, 8320, 9216, 9344, 11264, 12288, 14336, 16384])
+@pytest.mark.parametrize("rt", [None, BF16, F32], ids=lambda t: str(t).replace("torch.", ""))
+def test_a_row_does_not_depend_on_how_many_there_are(K, rt):
+    """The number of rows decides over how many CTAs of how many warps a row is spread; the order of its sums stays the same."""
+    rows = 721
+    g = torch.Generator().manual_seed(K)
+    x = torch.randn(rows, K, generator=g).to(BF16).to(DEV)
+    r = None if rt is None else torch.randn(rows, K, generator=g).to(rt).to(DEV)
+    w = (1 + 0.3 * torch.randn(K, generator=g)).to(DEV)
+    whole = f.rmsnorm_quantize(x, w, residual=r)
+    M = 736
+    values = x.double() + (0 if r is None else r.double())
+    inv = (values / torch.sqrt((values * values).mean(1, keepdim=True) + 1e-6) * w.double()).view(rows, K // 128, 128).abs().amax(2) / 448.0
+    assert ((whole[1].view(K // 128, M)[:, :rows].t().double() - inv).abs() <= scale_roundings(K, False, r is not None) * U * inv).all()
+    for n in (1, 16, 241, 257, 369, 449, 529, 600):
+        m = (n + 15) // 16 * 16
+        part = f.rmsnorm_quantize(x[:n], w, residual=None if r is None else r[:n])
+        assert torch.equal(part[0].view(K, m)[:, :n], whole[0].view(K, M)[:, :n]), n
+        assert torch.equal(part[1].view(K // 128, m)[:, :n], whole[1].view(K // 128, M)[:, :n]), n
+        if r is not None:
+            assert torch.equal(part[2], whole[2][:n])
+    f.last_device_status()
