@@ -255,12 +255,14 @@ int fp8bs_quantize_block(const void* W, int w_is_bf16, void* B_out, float* b_sca
 
 /* Root-mean-square norm with the residual's addition in front of it and the GEMM's A operand behind it, one launch:
  *     s = X + residual (fp32);  residual_out = s in the residual's type;  y = s / sqrt(mean(s^2) + eps) * weight (fp32)
- *     a_scale_out[m + Mp*kb] = 1 / scale,  A_out[m + Mp*k] = e4m3fn(clamp(y * scale)),  scale as in fp8bs_quantize_rowwise
+ *     a_scale_out[m + Mp*kb] = 1 / scale,  A_out[m + Mp*k] = e4m3fn(clamp(y * scale)),  scale = fp8_max / max(|y|, 1e-12)
+ * as in fp8bs_quantize_rowwise, but not to the last bit of what that makes of y rounded to fp32: y is not rounded on its way, and 1 / x is a Newton
+ * step on the hardware's approximation (error 2^-24).  A byte differs where a value lies within a few roundings of the border of two.
  * The norm sees s before it is rounded to residual_out.  X is [rows, K] with a row pitch of ldx elements, residual (may be NULL:
  * no addition, residual_out is not written) [rows, K] with a pitch of ldr, residual_out [rows, K] without gaps; residual_out may be
  * the residual itself, or X itself if it has the same type, without gaps (ldr or ldx = K); any other overlap with them is refused.  Each of X, residual
  * and weight [K] is bf16 (its flag != 0) or fp32.  Any rows >= 1: Mp is rows rounded up to a multiple of 16, and the rows behind
- * the last are written as zeros (scale fp8_max / 1e-12), so that one token is an operand of 16 rows.  A row that holds a NaN or an
+ * the last are written as +0 (scale fp8_max / 1e-12), whatever the weight, so that one token is an operand of 16 rows.  A row that holds a NaN or an
  * infinity gets NaN bytes and scales where torch's arithmetic has NaN.  K a multiple of 128 (rows of more
  * than 16384 columns, in fp32 with an fp32 residual than 13312, are read twice); all pointers but a_scale_out 16-byte aligned,
  * and the pitches multiples of 16 bytes; 0 < fp8_max <= 448; eps >= 0.  Asynchronous on `stream`. */

@@ -77,3 +77,54 @@ def test_a_row_does_not_depend_on_how_many_there_are(K, rt):
         if r is not None:
             assert torch.equal(part[2], whole[2][:n])
     f.last_device_status()
+
+
+@pytest.mark.parametrize("fp8_max", [448.0, 240.0])
+def test_reciprocals_of_many_magnitudes(fp8_max):
+    """One value of 1 per block makes the mean 1 / 128 exactly, and the scale of a block its weight times sqrt(128): 1.5 roundings of the root, the product, and
+    the two reciprocals with a product between."""
+    KB = 128
+    K = 128 * KB
+    g = torch.Generator().manual_seed(1)
+    for _ in range(8):
+        x = torch.zeros(1, K, device=DEV)
+        x[:, ::128] = 1.0
+        w = torch.zeros(K)
+        w[::128] = torch.exp(torch.empty(KB).uniform_(-25.0, 60.0, generator=g)) * (1 + torch.rand(KB, generator=g))
+        w = w.to(DEV)
+        _, sc = f.rmsnorm_quantize(x, w, eps=0.0, fp8_max=fp8_max)
+        want = w[::128].double() * 128 ** 0.5 / fp8_max
+        got = sc.view(KB, 16)[:, 0].double()
+        assert ((got - want).abs() <= (1.5 + 1 + 3) * U * 1.001 * want).all(), float(((got - want).abs() / want).max() / U)
+
+
+def test_roots_of_many_magnitudes():
+    """Rows with one value v: the mean is v^2 / 128 with one rounding, eps adds one, the root's own 1.5; then the value over the root and as above."""
+    rows, K = 4096, 128
+    g = torch.Generator().manual_seed(2)
+    v = torch.exp(torch.empty(rows).uniform_(-30.0, 40.0, generator=g)) * (1 + torch.rand(rows, generator=g))
+    x = torch.zeros(rows, K)
+    x[:, 5] = v
+    for eps in (0.0, 1e-6, 3e5):
+        _, sc = f.rmsnorm_quantize(x.to(DEV), torch.full((K,), 1e6, device=DEV), eps=eps)
+        v64, e = v.double(), torch.tensor(eps, dtype=F32).double()
+        want = (1e6 * v64 / torch.sqrt(v64 * v64 / 128 + e)).clamp(min=1e-12) / 448.0
+        got = sc.cpu().double()
+        # the weight of 1e6 is exact in fp32; its product with v rounds once
+        assert ((got - want).abs() <= (1.0 + 1.5 + 1 + 1 + 3) * U * 1.001 * want).all(), (eps, float(((got - want).abs() / want).max() / U))
+
+
+def test_the_scales_of_quantize_rowwise_within_their_roundings():
+    """With a root of exactly 1 the norm hands its rows to the scaling of quantize_rowwise: the values of both are e4m3 steps of the same scales up to the
+    counted roundings, and no byte is more than one step apart."""
+    rows, K = 64, 1024
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(rows, K, generator=g).to(DEV)
+    y = x.double() / torch.sqrt((x.double() ** 2).mean(1, keepdim=True) + 1e-6)
+    a, s = f.rmsnorm_quantize(x, torch.ones(K, device=DEV))
+    b, t = f.quantize_rowwise(y.float())
+    tol = (scale_roundings(K, False, False) + 4) * U          # and y's own rounding and three of the other scale
+    assert ((s.double() - t.double()).abs() <= tol * t.double()).all()
+    # magnitudes of e4m3 bytes are in order: neighbouring values have neighbouring bytes
+    assert ((a & 0x7F).int() - (b & 0x7F).int()).abs().max() <= 1
+    assert (((a ^ b) & 0x80 == 0) | ((a & 0x7F) == 0) | ((b & 0x7F) == 0)).all()
