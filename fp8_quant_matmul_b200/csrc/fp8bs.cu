@@ -462,9 +462,9 @@ static Config plan(const DeviceModel& dm, int device, int M, int N, int K, int p
 // ahead: 2.2 us per wave (0.3 on 128-wide tiles).  silu and bias, pair / 128-wide: 2960 x 1920 x 640 15.4 / 12.5 us, 6720 x 1488 x 512 20.2 / 17.4,
 // 4096 x 7168 x 512 38.3 / 35.1, 6144 x 4608 x 1024 42.4 / 44.7, 1440 x 1664 x 2304 14.6 / 15.6.  Gated, all are wide.
 // The estimate's overhead of the cluster reduction on 256-wide tiles is 1.5 us too much since the sums are sent to the CTA that finishes
-// them: gated 112 x 496 x 2048 took 12.8 us with it instead of 9.9, 144 x 1664 x 3584 15.0 instead of 13.7; on 60 shapes of up to 3000 rows the
-// choice is 1.2 % behind the best configuration of each, with it 2.3 %.  For bias and activation, where there are 128-wide tiles too, it is as
-// good without (1.0 %).  gemm() keeps its choices, and with them the order in which it adds.
+// them: gated 112 x 496 x 2048 took 12.8 us with it instead of 9.9, 144 x 1664 x 3584 15.0 instead of 13.7.  For bias and activation, where there are
+// 128-wide tiles too, it is as good without.  On 36 and 40 shapes of 65 to 3000 rows the choice is 1.5 % (gated) and 1.6 % (bias, activation) behind the best
+// configuration of each, 6 and 12 % at most (profiles/fused_choice.md).  gemm() keeps its choices, and with them the order in which it adds.
 static int choose_fused(const DeviceModel& dm, int M, int N, int K, bool gated, bool activation, int splits, int tile_n, Config* out)
 {
     const int KB = K / 128, t = tile_n & ~FP8BS_SMALL_M;

@@ -125,7 +125,8 @@ struct GemmParams {
 // over as one part, and its column group g takes columns 64 g .. of each slab.  A tile is exactly one scale block of h wide: its
 // two column groups exchange their rows' largest magnitudes through shared memory.
 // Bound by the K loop, as the product alone is; the epilogue's instructions are not hidden (the promotion warps issue them between two K
-// loops), its bytes are.  Measured: bias, gelu_tanh and residual on 6144 x 4608 x 7168 177-180 us (gemm() 160 in a short run, 182 at the power limit);
+// loops), its bytes are.  Measured: bias, gelu_tanh and residual on 6144 x 4608 x 7168 181 us in a short run, where gemm() takes 160;
+// in a loop at the power limit 211 at 1380 MHz (292 thousand cycles) and gemm() 190 at 1282 (244 thousand);
 // gated 4096 x 2048 x 7168 to bytes 103 (gemm() on 4096 x 4096 x 7168 98), 192 x 2304 x 7168 in three splits 19.8 (gemm() on 192 x 4608 x 7168
 // 14.8 on 128-wide tiles, which a gated scale block does not fit).
 enum : int { EPI_NONE = 0, EPI_BIAS_ACT = 1, EPI_GATED = 2, EPI_GATED_FP8 = 3 };

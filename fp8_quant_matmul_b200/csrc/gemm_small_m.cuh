@@ -76,12 +76,12 @@ __device__ __forceinline__ void tmem_ld_x32_sync(uint32_t taddr, uint32_t (&v)[3
         : "memory");
 }
 
-// grid = n_tiles * splits CTAs, cluster size = splits.
 // The second matrix of the gated form; no parameter otherwise.
 struct NoMap {};
 template <int EPI>
 using SecondMap = typename std::conditional<EPI == EPI_GATED || EPI == EPI_GATED_FP8, CUtensorMap, NoMap>::type;
 
+// grid = n_tiles * splits CTAs, cluster size = splits.
 template <int T, int EPI = EPI_NONE>
 __global__ void __launch_bounds__((SmallMCfg<T, EPI>::THREADS), (SmallMCfg<T, EPI>::CTAS))
 gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const GemmParams p,
@@ -227,12 +227,11 @@ gemm_small_m_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                     a[i] = m < p.M ? __ldg(p.a_scale + static_cast<size_t>(fkb) * p.M + m) : 0.0f;
                 }
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    {
-                        const float* bp = p.b_scale;
-                        if constexpr (GATED) bp = h ? ea.e.up_scale : bp;
-                        b[h] = __ldg(bp + static_cast<size_t>(fkb) * p.sn + nb[GATED ? 0 : h]) * p.elem_scale;
-                    }
+                for (int h = 0; h < 2; ++h) {
+                    const float* bp = p.b_scale;
+                    if constexpr (GATED) bp = h ? ea.e.up_scale : bp;
+                    b[h] = __ldg(bp + static_cast<size_t>(fkb) * p.sn + nb[GATED ? 0 : h]) * p.elem_scale;
+                }
             }
             ++fkb;
         };

@@ -15,10 +15,11 @@
 // box is requested as soon as this one is in registers.  The warps of a CTA have nothing else to do with one another; with copies per row for the
 // CTA as a whole, two barriers and sums per CTA a round took up to 15 % longer.
 // Measured (CUDA graph, cold inputs, outputs of their own): 4096 x 7168 bf16 43-44 us with residual (206 MB: 4.7 TB/s; a copy reaches 6.4), 28
-// without (3.2 TB/s); 6144 x 4608 bf16 with residual 39 (5.1), fp32 with residual 67 (5.5); one row of 7168 3.4, with residual 4.1, the chain of a
+// without (3.2 TB/s); 6144 x 4608 bf16 with residual 39 (5.1), fp32 with residual 67 (5.5); one row of 7168 3.3, with residual 3.9, the chain of a
 // launch and one round.  What bounds it: in bf16 the instructions of a round and the waits between them, 16 warps per SM at most
 // with 128 registers each; in fp32 nearly the memory.
-// Rows that do not fit (more than 16384 columns; in fp32 with an fp32 residual more than 13312) are read twice.
+// Rows that do not fit (more than 16384 columns; in fp32 with an fp32 residual more than 13312) are read twice: 512 x
+// 20480 bf16 23-24 us, with residual 34-35 (5.0 and 11.5 at a copy's rate, reading once).
 #pragma once
 #include "quantize.cuh"
 #include <type_traits>
