@@ -464,7 +464,7 @@ static Config plan(const DeviceModel& dm, int device, int M, int N, int K, int p
 // The estimate's overhead of the cluster reduction on 256-wide tiles is 1.5 us too much since the sums are sent to the CTA that finishes
 // them: gated 112 x 496 x 2048 took 12.8 us with it instead of 9.9, 144 x 1664 x 3584 15.0 instead of 13.7.  For bias and activation, where there are
 // 128-wide tiles too, it is as good without.  On 36 and 40 shapes of 65 to 3000 rows the choice is 1.5 % (gated) and 1.6 % (bias, activation) behind the best
-// configuration of each, 6 and 12 % at most (profiles/fused_choice.md).  gemm() keeps its choices, and with them the order in which it adds.
+// configuration of each, 6 and 12 % at most.  gemm() keeps its choices, and with them the order in which it adds.
 static int choose_fused(const DeviceModel& dm, int M, int N, int K, bool gated, bool activation, int splits, int tile_n, Config* out)
 {
     const int KB = K / 128, t = tile_n & ~FP8BS_SMALL_M;
@@ -804,7 +804,9 @@ static int launch_rmsnorm(NormParams p, const DeviceInfo* dev, cudaStream_t st)
         warps = least <= 8 ? equal_shares(11) : ceil_div(KB, 6) <= NORM_MOST_WARPS ? ceil_div(KB, 6) : least;
         for (int c = NORM_MAX_CLUSTER; c >= 4 && ceil_div(KB, c) <= NORM_MOST_WARPS; --c) {
             const int w = ceil_div(KB, c), cluster = ceil_div(KB, w), alone = dev->model.max_clusters[cluster];
-            if ((rc = norm_clusters<X, R>(device, cluster, w, static_cast<int>(smem_of(w)), &most))) return rc;
+            rc = norm_clusters<X, R>(device, cluster, w, static_cast<int>(smem_of(w)), &most);
+            if (rc == FP8BS_ERR_NO_DEVICE) continue;                             // a part of a GPU that has no room for such a cluster
+            if (rc) return rc;
             const int r = ceil_div(groups, most), o = groups > alone && most >= 2 * alone ? 2 * w : w;
             if (r < rounds || (r == rounds && r < 3 && o < on_sm)) {
                 rounds = r;
